@@ -233,5 +233,6 @@ class BitCache:
 
 
 from bitcache_amd import functional  # noqa: E402,F401
+from bitcache_amd.paged import PagedBitCache  # noqa: E402
 
-__all__ = ["BitCache", "functional", "default_top_k"]
+__all__ = ["BitCache", "PagedBitCache", "functional", "default_top_k"]

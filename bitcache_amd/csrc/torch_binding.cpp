@@ -652,6 +652,202 @@ torch::Tensor reference_attention(torch::Tensor Q, torch::Tensor K, torch::Tenso
     return out.view(Q.sizes());
 }
 
+// ------------------------------------------------------------------ pages
+// Rows of queries, keys or values [tokens, heads, head_dim], fp16 or bf16, unit
+// stride in the last dim (a slice of a fused projection is one).
+void check_rows(const torch::Tensor& x, const char* name) {
+    TORCH_CHECK(x.device().is_cuda(), name, " must be a ROCm (cuda) tensor");
+    TORCH_CHECK(x.scalar_type() == torch::kFloat16 || x.scalar_type() == torch::kBFloat16, name,
+                " must be float16 or bfloat16");
+    TORCH_CHECK(x.dim() == 3, name, " must be 3D [tokens, heads, head_dim]");
+    TORCH_CHECK(x.numel() == 0 || x.size(2) == 1 || x.stride(2) == 1, name, " must have unit stride in the last dim");
+    TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()), name,
+                " requires a gradient, and this operator has none (use torch.no_grad() or detach())");
+}
+
+void check_like(const torch::Tensor& x, const torch::Tensor& a, const char* name) {
+    check_rows(x, name);
+    TORCH_CHECK(x.scalar_type() == a.scalar_type(), name, " must have the dtype of the other rows");
+    TORCH_CHECK(x.device() == a.device(), name, " must be on the same device as the other rows");
+    TORCH_CHECK(x.size(0) == a.size(0) && x.size(2) == a.size(2), name,
+                " must hold the other rows' tokens and head_dim");
+}
+
+int bc_dtype_of(const torch::Tensor& x) { return x.scalar_type() == torch::kBFloat16 ? BC_BF16 : BC_FP16; }
+
+int as_int(int64_t v, const char* name) {
+    TORCH_CHECK(v >= 0 && v <= INT32_MAX, name, " must be 0 to 2^31 - 1, got ", v);
+    return (int)v;
+}
+
+// An index vector of the tokens (int64), or a table of the sequences (int32).
+void check_index(const torch::Tensor& x, const torch::Tensor& rows, torch::ScalarType type, const char* name) {
+    TORCH_CHECK(x.device() == rows.device(), name, " must be on the rows' device");
+    TORCH_CHECK(x.scalar_type() == type, name, " must be ", type == torch::kInt64 ? "int64" : "int32");
+    TORCH_CHECK(x.is_contiguous(), name, " must be contiguous");
+}
+
+// The rotation of a call: positions [tokens] int64, cos and sin [table, rot/2]
+// float32 (all or none), and the norms' weights [head_dim].
+struct Rotation {
+    const int64_t* positions = nullptr;
+    const float *cos = nullptr, *sin = nullptr;
+    const void *qw = nullptr, *kw = nullptr;
+    int64_t table = 0;
+    int rot = 0;
+};
+
+Rotation rotation_of(const torch::Tensor& rows, const std::optional<torch::Tensor>& positions,
+                     const std::optional<torch::Tensor>& cos, const std::optional<torch::Tensor>& sin,
+                     const std::optional<torch::Tensor>& q_weight, const std::optional<torch::Tensor>& k_weight) {
+    Rotation r;
+    TORCH_CHECK(positions.has_value() == cos.has_value() && cos.has_value() == sin.has_value(),
+                "positions, cos and sin: all or none");
+    if (positions.has_value()) {
+        check_index(*positions, rows, torch::kInt64, "positions");
+        TORCH_CHECK(positions->dim() == 1 && positions->size(0) == rows.size(0), "positions must be [tokens]");
+        for (const auto* t : {&*cos, &*sin}) {
+            TORCH_CHECK(t->device() == rows.device() && t->scalar_type() == torch::kFloat32 && t->is_contiguous() &&
+                            t->dim() == 2,
+                        "cos and sin must be contiguous float32 [table, rot_dim / 2] on the rows' device");
+            TORCH_CHECK(!(t->requires_grad() && at::GradMode::is_enabled()), "cos and sin have no gradient");
+        }
+        TORCH_CHECK(cos->sizes() == sin->sizes(), "cos and sin must have the same shape");
+        TORCH_CHECK(cos->size(0) > 0, "cos and sin hold no position");
+        r.rot = as_int(2 * cos->size(1), "rot_dim");
+        TORCH_CHECK(r.rot > 0 && r.rot % 16 == 0 && r.rot <= rows.size(2),
+                    "rot_dim (2 * cos.size(1)) must be a multiple of 16 up to head_dim, got ", r.rot);
+        r.positions = positions->data_ptr<int64_t>();
+        r.cos = cos->data_ptr<float>();
+        r.sin = sin->data_ptr<float>();
+        r.table = cos->size(0);
+    }
+    auto weight = [&](const std::optional<torch::Tensor>& w, const char* name) -> const void* {
+        if (!w.has_value()) return nullptr;
+        TORCH_CHECK(w->device() == rows.device() && w->scalar_type() == rows.scalar_type() && w->is_contiguous() &&
+                        w->dim() == 1 && w->size(0) == rows.size(2),
+                    name, " must be contiguous [head_dim] with the rows' dtype and device");
+        TORCH_CHECK(!(w->requires_grad() && at::GradMode::is_enabled()), name,
+                    " requires a gradient, and this operator has none (use torch.no_grad() or detach())");
+        return w->data_ptr();
+    };
+    r.qw = weight(q_weight, "q_weight");
+    r.kw = weight(k_weight, "k_weight");
+    return r;
+}
+
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> norm_rotary(
+    torch::Tensor q, std::optional<torch::Tensor> k, std::optional<torch::Tensor> positions,
+    std::optional<torch::Tensor> cos, std::optional<torch::Tensor> sin, std::optional<torch::Tensor> q_weight,
+    std::optional<torch::Tensor> k_weight, double eps, bool interleaved) {
+    check_rows(q, "q");
+    if (k.has_value()) check_like(*k, q, "k");
+    const Rotation r = rotation_of(q, positions, cos, sin, q_weight, k_weight);
+    TORCH_CHECK(k.has_value() || r.kw == nullptr, "k_weight without keys");
+    c10::DeviceGuard guard(q.device());
+    auto q_out = torch::empty(q.sizes(), q.options());
+    std::optional<torch::Tensor> k_out;
+    if (k.has_value()) k_out = torch::empty(k->sizes(), k->options());
+    check_status(bc_norm_rotary(q.data_ptr(), q.stride(0), q.stride(1), k ? k->data_ptr() : nullptr,
+                                k ? k->stride(0) : 0, k ? k->stride(1) : 0, r.positions, r.cos, r.sin, r.table,
+                                r.qw, r.kw, eps, q_out.data_ptr(), k_out ? k_out->data_ptr() : nullptr, q.size(0),
+                                as_int(q.size(1), "n_heads"), k ? as_int(k->size(1), "n_kv_heads") : 0,
+                                as_int(q.size(2), "head_dim"), r.rot, interleaved ? 1 : 0, bc_dtype_of(q),
+                                stream_of(q)),
+                 "norm_rotary");
+    return {q_out, k_out};
+}
+
+// The pools of a paged cache: pointers and the pages they hold.
+struct Pools {
+    void *kb, *kr = nullptr, *vb, *vr = nullptr;
+    int n_pages;
+};
+
+Pools pools_of(const torch::Tensor& rows, const torch::Tensor& K_bin, const std::optional<torch::Tensor>& K_res,
+               const torch::Tensor& V_bin, const std::optional<torch::Tensor>& V_res, int64_t n_kv_heads,
+               int64_t page_size) {
+    TORCH_CHECK(n_kv_heads > 0 && page_size > 0 && page_size % 64 == 0,
+                "page_size must be a multiple of 64 and n_kv_heads > 0");
+    TORCH_CHECK(K_res.has_value() == V_res.has_value(), "K_res and V_res: both or neither");
+    check_same_device(rows, K_bin, "K_bin");
+    check_same_device(rows, V_bin, "V_bin");
+    Pools p;
+    const int64_t cap = resolve_blob(K_bin, bc_sizeof_binary_vec(), "K_bin").cap;
+    TORCH_CHECK(cap % (n_kv_heads * page_size) == 0, "K_bin holds ", cap, " vectors: not whole pages of ", page_size,
+                " slots and ", n_kv_heads, " heads");
+    p.n_pages = as_int(cap / (n_kv_heads * page_size), "n_pages");
+    p.kb = blob_exact(K_bin, cap, bc_sizeof_binary_vec(), "K_bin");
+    p.vb = blob_exact(V_bin, cap, bc_sizeof_binary_vec(), "V_bin");
+    if (K_res.has_value()) {
+        check_same_device(rows, *K_res, "K_res");
+        check_same_device(rows, *V_res, "V_res");
+        p.kr = blob_exact(*K_res, cap, bc_sizeof_residual_vec(), "K_res");
+        p.vr = blob_exact(*V_res, cap, bc_sizeof_residual_vec(), "V_res");
+    }
+    return p;
+}
+
+std::optional<torch::Tensor> paged_append(
+    std::optional<torch::Tensor> q, torch::Tensor k, torch::Tensor v, std::optional<torch::Tensor> positions,
+    torch::Tensor slots, std::optional<torch::Tensor> cos, std::optional<torch::Tensor> sin, torch::Tensor K_bin,
+    std::optional<torch::Tensor> K_res, torch::Tensor V_bin, std::optional<torch::Tensor> V_res, int64_t page_size,
+    std::optional<torch::Tensor> q_weight, std::optional<torch::Tensor> k_weight, double eps, bool interleaved) {
+    check_rows(k, "k");
+    check_like(v, k, "v");
+    TORCH_CHECK(v.size(1) == k.size(1), "k and v must have the same heads");
+    if (q.has_value()) check_like(*q, k, "q");
+    check_index(slots, k, torch::kInt64, "slots");
+    TORCH_CHECK(slots.dim() == 1 && slots.size(0) == k.size(0), "slots must be [tokens]");
+    const Rotation r = rotation_of(k, positions, cos, sin, q_weight, k_weight);
+    TORCH_CHECK(q.has_value() || r.qw == nullptr, "q_weight without queries");
+    const Pools p = pools_of(k, K_bin, K_res, V_bin, V_res, k.size(1), page_size);
+    c10::DeviceGuard guard(k.device());
+    std::optional<torch::Tensor> q_out;
+    if (q.has_value()) q_out = torch::empty(q->sizes(), q->options());
+    check_status(bc_paged_append(q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0,
+                                 k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                 r.positions, r.cos, r.sin, r.table, r.qw, r.kw, eps,
+                                 q_out ? q_out->data_ptr() : nullptr, slots.data_ptr<int64_t>(), p.kb, p.kr, p.vb,
+                                 p.vr, p.n_pages, as_int(page_size, "page_size"), k.size(0),
+                                 q ? as_int(q->size(1), "n_heads") : 0, as_int(k.size(1), "n_kv_heads"),
+                                 as_int(k.size(2), "head_dim"), r.rot, interleaved ? 1 : 0, bc_dtype_of(k),
+                                 stream_of(k)),
+                 "paged_append");
+    return q_out;
+}
+
+torch::Tensor paged_attention(torch::Tensor Q, torch::Tensor K_bin, std::optional<torch::Tensor> K_res,
+                              torch::Tensor V_bin, std::optional<torch::Tensor> V_res, torch::Tensor block_tables,
+                              torch::Tensor seq_lens, int64_t n_kv_heads, int64_t page_size, int64_t max_seq_len,
+                              int64_t shared_len) {
+    check_rows(Q, "Q");
+    BC_CHECK_CONTIG(Q);
+    const int64_t batch = Q.size(0), n_heads = Q.size(1), d = Q.size(2);
+    TORCH_CHECK(n_kv_heads > 0 && n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
+    check_index(block_tables, Q, torch::kInt32, "block_tables");
+    check_index(seq_lens, Q, torch::kInt32, "seq_lens");
+    TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == batch, "block_tables must be [batch, pages]");
+    TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == batch, "seq_lens must be [batch]");
+    const Pools p = pools_of(Q, K_bin, K_res, V_bin, V_res, n_kv_heads, page_size);
+    c10::DeviceGuard guard(Q.device());
+    size_t ws_bytes = 0;
+    check_status(bc_paged_attention_workspace_size(as_int(batch, "batch"), as_int(n_heads, "n_heads"),
+                                                   as_int(n_kv_heads, "n_kv_heads"),
+                                                   as_int(max_seq_len, "max_seq_len"),
+                                                   as_int(shared_len, "shared_len"), as_int(d, "head_dim"), &ws_bytes),
+                 "paged_attention_workspace_size");
+    auto ws = workspace_for(Q, ws_bytes);
+    auto out = torch::empty({batch, n_heads, d}, Q.options());
+    check_status(bc_paged_attention(Q.data_ptr(), p.kb, p.kr, p.vb, p.vr, block_tables.data_ptr<int32_t>(),
+                                    as_int(block_tables.size(1), "table width"), seq_lens.data_ptr<int32_t>(),
+                                    out.data_ptr(), (int)batch, (int)n_heads, (int)n_kv_heads, p.n_pages,
+                                    as_int(page_size, "page_size"), (int)max_seq_len, (int)shared_len, (int)d,
+                                    bc_dtype_of(Q), ws.data_ptr(), ws_bytes, stream_of(Q)),
+                 "paged_attention");
+    return out;
+}
+
 // ------------------------------------------------------------------ format conversion
 torch::Tensor convert(torch::Tensor blob, int64_t n, int64_t head_dim, bool residual, bool to_ref) {
     const int64_t per = residual ? bc_sizeof_residual_vec() : bc_sizeof_binary_vec();
@@ -714,5 +910,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("binary_scores", &binary_scores, "Exact per-key binary scores and popcounts");
     m.def("adaptive_select", &adaptive_select, "entropy >= threshold ? 0 (binary) : 1");
     m.def("reference_attention", &reference_attention, "Exact fp16 attention (fp32 accumulation)");
+    m.def("norm_rotary", &norm_rotary, "Norms of query and key heads with the position rotation");
+    m.def("paged_append", &paged_append, "New tokens, rotated and encoded, into a paged cache");
+    m.def("paged_attention", &paged_attention, "Decode attention over pages, a length per sequence");
     m.def("convert", &convert, "Dense planar blob <-> reference array-of-structs bytes");
 }

@@ -175,6 +175,71 @@ def reference_attention(Q: Tensor, K: Tensor, V: Tensor, batch: int, n_heads: in
                                   n_heads if n_kv_heads is None else n_kv_heads, seq_len, head_dim)
 
 
+def norm_rotary(q: Tensor, k: Optional[Tensor], positions: Optional[Tensor],
+                cos: Optional[Tensor], sin: Optional[Tensor], *, q_weight: Optional[Tensor] = None,
+                k_weight: Optional[Tensor] = None, eps: float = 1e-6,
+                interleaved: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """Norms of query and key heads with the position rotation in the same pass: what a
+    decode step does between the projections and append_attend(k, v, q).
+
+    q [tokens, n_heads, d], k [tokens, n_kv_heads, d] (or None): fp16 or bf16, slices of
+    a fused projection are fine (unit stride in the last dim).  With weights [d], each
+    row is x * weight / sqrt(mean x^2 + eps).  positions [tokens] int64 index the tables
+    cos, sin [table, rot_dim / 2] float32; the pairs (i, i + rot_dim / 2) of the first
+    rot_dim elements turn, or (2i, 2i + 1) when interleaved.  rot_dim is a multiple of
+    16 up to d; without positions, cos and sin the rows are only normed.  64-bit
+    arithmetic, rounded once.  A position outside the table gives NaN.  No gradient:
+    inputs that require one are refused.  Returns (q', k'), contiguous."""
+    _require_extension()
+    return _C.norm_rotary(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+
+
+def paged_append(k: Tensor, v: Tensor, slots: Tensor, K_bin: Tensor, K_res: Optional[Tensor],
+                 V_bin: Tensor, V_res: Optional[Tensor], page_size: int) -> None:
+    """Encode k, v [tokens, n_kv_heads, d] (fp16 or bf16) into slots [tokens] int64 of a
+    paged cache: slot = page * page_size + offset, the vector (page * n_kv_heads + head) *
+    page_size + offset of blobs of n_pages * n_kv_heads * page_size vectors.  The bytes of
+    a ring cache's append (online encode) of the same rows.  K_res / V_res None: signs
+    only.  A slot outside the pool (-1) is padding and goes nowhere; two tokens of a call
+    may not name the same slot.  page_size is a multiple of 64."""
+    _require_extension()
+    _C.paged_append(None, k, v, None, slots, None, None, K_bin, K_res, V_bin, V_res, page_size,
+                    None, None, 0.0, False)
+
+
+def rotary_append(q: Tensor, k: Tensor, v: Tensor, positions: Tensor, slots: Tensor, cos: Tensor,
+                  sin: Tensor, K_bin: Tensor, K_res: Optional[Tensor], V_bin: Tensor,
+                  V_res: Optional[Tensor], page_size: int, *, q_weight: Optional[Tensor] = None,
+                  k_weight: Optional[Tensor] = None, eps: float = 1e-6,
+                  interleaved: bool = False) -> Tensor:
+    """norm_rotary(q, k) and paged_append(k', v) in one launch, with their bytes; returns q'."""
+    _require_extension()
+    return _C.paged_append(q, k, v, positions, slots, cos, sin, K_bin, K_res, V_bin, V_res,
+                           page_size, q_weight, k_weight, eps, interleaved)
+
+
+def paged_attention(Q: Tensor, K_bin: Tensor, K_res: Optional[Tensor], V_bin: Tensor,
+                    V_res: Optional[Tensor], block_tables: Tensor, seq_lens: Tensor,
+                    max_seq_len: int, page_size: int, *, n_kv_heads: Optional[int] = None,
+                    shared_len: int = 0) -> Tensor:
+    """Decode attention over a paged cache (paged_append), a length per sequence.
+
+    Q [batch, n_heads, d] fp16 or bf16; block_tables [batch, pages] int32: sequence b's
+    key s is in page block_tables[b, s // page_size]; seq_lens [batch] int32, none above
+    max_seq_len.  K_res / V_res None: binary attention, else compensated.  Lengths and
+    tables are read on the device only (a captured call follows them).  Length 0 or less:
+    zeros.  A length above max_seq_len or the table, or a page outside the pool among the
+    keys of a sequence: NaN for that sequence.
+
+    shared_len (whole pages): the first shared_len keys of every sequence are the same
+    pages, as behind a common prompt; they are read from the first row of block_tables and
+    attended once for the whole batch.  The result is that of shared_len = 0."""
+    _require_extension()
+    return _C.paged_attention(Q, K_bin, K_res, V_bin, V_res, block_tables, seq_lens,
+                              Q.shape[1] if n_kv_heads is None else n_kv_heads, page_size,
+                              max_seq_len, shared_len)
+
+
 def sizeof_binary_vec() -> int:
     _require_extension()
     return _C.sizeof_binary_vec()

@@ -315,6 +315,73 @@ int bc_adaptive_attention(const void* q, const void* k_bin, const void* k_res, c
                           int n_heads, int n_kv_heads, int seq_len, int kv_stride, int head_dim,
                           int top_k, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- pages ------------------------------------------------------------------ */
+/* A paged cache is a binary (and a residual) blob of n_pages * n_kv_heads *
+ * page_size vectors: vector (page * n_kv_heads + kv_head) * page_size + offset
+ * is the key or value of that head in slot page * page_size + offset.
+ * page_size is a multiple of 64 (the keys of an attention tile), so a tile
+ * never spans two pages.  Rows of queries, keys and values are fp16 or bf16
+ * (dtype), [tokens, heads, head_dim] with unit stride in the last dim and
+ * strides in elements in the others (a slice of a fused projection). */
+enum bc_dtype { BC_FP16 = 0, BC_BF16 = 1 };
+
+/* Norms of query and key heads with the position rotation in the same pass:
+ * a row x becomes y = x * weight / sqrt(mean x^2 + eps) (weight [head_dim] of the
+ * rows' type; null: y = x), then the pairs (i, i + rot_dim/2) (interleaved:
+ * (2i, 2i+1)) of its first rot_dim elements turn by the angle of the token's
+ * position: (y1 c - y2 s, y2 c + y1 s), c = cos[position][i], s = sin[position][i]
+ * (fp32 tables [table_len, rot_dim/2]).  rot_dim a multiple of 16; positions,
+ * cos and sin null: norms alone.  Products and sums in 64 bits, one rounding
+ * to the rows' type.  A position outside the table gives NaN.  n_kv_heads 0:
+ * queries only.  Outputs are contiguous.  No counterpart in the reference. */
+int bc_norm_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                   int64_t k_token_stride, int64_t k_head_stride, const int64_t* positions,
+                   const float* cos, const float* sin, int64_t table_len, const void* q_weight,
+                   const void* k_weight, double eps, void* q_out, void* k_out, int64_t n_tokens,
+                   int n_heads, int n_kv_heads, int head_dim, int rot_dim, int interleaved,
+                   int dtype, void* stream);
+
+/* New tokens into a paged cache, in one launch: keys (after the norm and
+ * rotation of bc_norm_rotary, rounded to the rows' type) and values are encoded
+ * into slot slots[t] with the online-encode math (the bytes of
+ * bc_online_encode_kv of the same rows), and the queries' rows are written to
+ * q_out.  n_heads 0: keys and values only; positions null: no rotation;
+ * k_res / v_res both null: binary cache.  A slot outside [0, n_pages *
+ * page_size) is padding: the token's key and value go nowhere.  Two tokens of
+ * a call may not name the same slot (its record is then undefined).  No
+ * counterpart in the reference (its caches are rings,
+ * src/online_encode.cu:122-149). */
+int bc_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                    int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                    int64_t v_token_stride, int64_t v_head_stride, const int64_t* positions,
+                    const float* cos, const float* sin, int64_t table_len, const void* q_weight,
+                    const void* k_weight, double eps, void* q_out, const int64_t* slots,
+                    void* k_bin, void* k_res, void* v_bin, void* v_res, int n_pages, int page_size,
+                    int64_t n_tokens, int n_heads, int n_kv_heads, int head_dim, int rot_dim,
+                    int interleaved, int dtype, void* stream);
+
+/* Decode attention over a paged cache, a length per sequence: q, out [batch,
+ * n_heads, head_dim] (contiguous, dtype), sequence b attends to its first
+ * seq_lens[b] keys, key s in slot block_tables[b * table_width + s / page_size]
+ * * page_size + s % page_size.  Scores and values as bc_attention_gqa (k_res /
+ * v_res both null: binary attention).  max_seq_len: no length is larger (the
+ * launch is planned for it; it may be larger than every length).  Lengths and
+ * tables are read on the device, so a captured call follows them.  A length of
+ * 0 or less gives zeros.  A length above max_seq_len or the table's width, or a
+ * page outside [0, n_pages) among a sequence's keys gives NaN for that
+ * sequence; nothing outside the cache is read.
+ * shared_len (whole pages; 0: none): the first shared_len keys of every sequence
+ * are the same pages (read from the first row of block_tables), attended once
+ * for all sequences.  The result is that of shared_len 0.
+ * No counterpart in the reference. */
+int bc_paged_attention_workspace_size(int batch, int n_heads, int n_kv_heads, int max_seq_len,
+                                      int shared_len, int head_dim, size_t* bytes);
+int bc_paged_attention(const void* q, const void* k_bin, const void* k_res, const void* v_bin,
+                       const void* v_res, const int32_t* block_tables, int table_width,
+                       const int32_t* seq_lens, void* out, int batch, int n_heads, int n_kv_heads,
+                       int n_pages, int page_size, int max_seq_len, int shared_len, int head_dim,
+                       int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Exact fp16 attention with fp32 accumulation over dense K/V
  * [batch, n_kv_heads, seq_len, head_dim] (the speed baseline and GPU oracle).
  * Workspace from bc_attention_workspace_size().
