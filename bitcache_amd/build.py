@@ -28,7 +28,8 @@ EXT_SUFFIX = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
 EXT = os.path.join(HERE, "_C" + EXT_SUFFIX)
 
 # (the longest compiles first: the matrix-core attention kernels, one file per head dim)
-HIP_SOURCES = [f"attn_mfma_d{d}.hip" for d in (256, 224, 192, 160, 128, 96, 64, 32)] + [
+HIP_SOURCES = [f"attn_{kind}_d{d}.hip" for d in (256, 224, 192, 160, 128, 96, 64, 32)
+               for kind in ("mfma", "paged")] + [
     "attention.hip", "adaptive.hip", "encode.hip", "rotary.hip", "paged.hip", "attention_mfma.hip", "convert.hip", "probe.hip", "abi.cpp"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",

@@ -1245,6 +1245,8 @@ void launch_combine(const float* ws, uint16_t* out, int bh, int n_splits, hipStr
 
 namespace bc {
 
+int attention_group(int group, int D, int mode) { return attn_g(group, D, mode); }
+
 // Phase 1 (split partials into the workspace) and phase 2 (combine).  Shared
 // by the public entry points and the adaptive driver (adaptive.hip).
 int run_partial(int mode, const void* q, const void* k_bin, const void* k_res, const void* v_bin,

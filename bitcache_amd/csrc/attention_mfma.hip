@@ -13,21 +13,23 @@ namespace bc {
 
 #define BC_MFMA_EXTERN(D)                                                                              \
     extern template bool mfma_launch<D>(int, int, const AttnArgs&, dim3, hipStream_t, int);            \
-    extern template int mfma_occupancy<D>(int, int);
+    extern template int mfma_occupancy<D>(int, int);                                                   \
+    extern template void paged_launch<D>(int, int, const AttnArgs&, dim3, hipStream_t);                \
+    extern template int paged_occupancy<D>(int, int);
 BC_MFMA_DIMS(BC_MFMA_EXTERN)
 
-int mfma_wgs_per_cu(int mode, int D, int G) {
+static int wgs_per_cu(int mode, int D, int G, bool paged) {
     static std::mutex mu;
-    static std::map<std::tuple<int, int, int, int>, int> cache;
+    static std::map<std::tuple<int, int, int, int, bool>, int> cache;
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return 0;
-    const auto key = std::make_tuple(dev, mode, D, G);
+    const auto key = std::make_tuple(dev, mode, D, G, paged);
     std::lock_guard<std::mutex> lock(mu);
     const auto it = cache.find(key);
     if (it != cache.end()) return it->second;
     int n = 0;
     switch (D) {
-#define BC_MFMA_CASE(DD) case DD: n = mfma_occupancy<DD>(mode, G); break;
+#define BC_MFMA_CASE(DD) case DD: n = paged ? paged_occupancy<DD>(mode, G) : mfma_occupancy<DD>(mode, G); break;
         BC_MFMA_DIMS(BC_MFMA_CASE)
 #undef BC_MFMA_CASE
         default: n = 0;
@@ -36,6 +38,9 @@ int mfma_wgs_per_cu(int mode, int D, int G) {
     return n;
 }
 
+int mfma_wgs_per_cu(int mode, int D, int G) { return wgs_per_cu(mode, D, G, false); }
+int paged_wgs_per_cu(int mode, int D, int G) { return wgs_per_cu(mode, D, G, true); }
+
 bool mfma_split_ok(int D, int64_t chunk, int64_t head_groups) {
     if (!head_dim_ok(D) || head_groups > kMaxHeadGroups) return false;
     // buffer offsets are 32-bit and relative to a split's key range; the
@@ -43,6 +48,15 @@ bool mfma_split_ok(int D, int64_t chunk, int64_t head_groups) {
     // value path adds at most 2^16 per tile to an int32 accumulator: a wave
     // takes at most 2^15 tiles (a split below 2^23 keys)
     return (chunk + 2048) * (D / 2) + 4096 < ((int64_t)1 << 31) && chunk < ((int64_t)1 << 23);
+}
+
+bool launch_paged_split(int mode, int D, int G, const AttnArgs& a, dim3 grid, hipStream_t st) {
+    switch (D) {
+#define BC_MFMA_CASE(DD) case DD: paged_launch<DD>(mode, G, a, grid, st); return true;
+        BC_MFMA_DIMS(BC_MFMA_CASE)
+#undef BC_MFMA_CASE
+        default: return false;
+    }
 }
 
 bool launch_mfma_split(int mode, int D, int G, const AttnArgs& a, dim3 grid, hipStream_t st, int nw) {

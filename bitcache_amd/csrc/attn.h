@@ -47,7 +47,95 @@ struct AttnArgs {
     // normalised output [B, Hq, D] fp16 here instead of its partial, and no
     // merge launch follows
     uint16_t* out;
+    // paged caches: sequence b's keys are the first lens[b] of the pages
+    // tables[b * width + i], page_tiles 64-key tiles each (a null lens: no
+    // pages).  Keys before key0 (a shared prefix) are attended elsewhere.
+    const int32_t* lens;
+    const int32_t* tables;
+    int width, n_pages, page_tiles, key0, max_len;
+    int unit_tiles;   // see PagedUnit; 0: one unit per sequence
+    int unit_target;
+    int bf16;         // queries and outputs are bf16
 };
+
+// Work units of a paged call: a sequence's tiles after key0 are cut into units of
+// equal size, as many as bring a unit to at most `chunk` tiles, where chunk is
+// the batch's tiles over unit_target units, at least unit_tiles (and at most
+// kUnitTiles: a wave holds its tiles' places in one register).  A batch of
+// any lengths then is at most max(unit_target, batch * tiles / kUnitTiles) +
+// batch units of nearly the same size, and the launch is planned without
+// knowing the lengths.  unit_tiles = 0: unit b is sequence b.  Each wave finds its unit by
+// itself from the lengths (one load per 64 sequences and two wave scans).
+constexpr int kUnitTiles = 256;
+struct PagedUnit {
+    int b, len;        // (b < 0: no such unit)
+    int first, tiles;  // the unit's tiles, counted from key0
+};
+// A length that no bound or table holds
+__host__ __device__ inline bool paged_bad_len(const AttnArgs& a, int len) {
+    return len > a.max_len || (int64_t)len > (int64_t)a.width * a.page_tiles * 64;
+}
+__device__ __forceinline__ int paged_tiles(const AttnArgs& a, int len) {
+    return len <= a.key0 || paged_bad_len(a, len) ? 0 : (len - a.key0 + 63) / 64;
+}
+// Inclusive sum over the wave's lanes
+__device__ __forceinline__ int wave_scan_add(int v) {
+#define BC_SCAN_STEP(CTRL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+    BC_SCAN_STEP(0x111, 0xF)   // row_shr 1, 2, 4, 8
+    BC_SCAN_STEP(0x112, 0xF)
+    BC_SCAN_STEP(0x114, 0xF)
+    BC_SCAN_STEP(0x118, 0xF)
+    BC_SCAN_STEP(0x142, 0xA)   // row broadcasts into the rows after
+    BC_SCAN_STEP(0x143, 0xC)
+#undef BC_SCAN_STEP
+    return v;
+}
+// Tiles of a unit at most
+__device__ __forceinline__ int paged_chunk(const AttnArgs& a, int lane) {
+    int n = 0;
+    for (int i = lane; i < a.B; i += 64) n += paged_tiles(a, a.lens[i]);
+    const int total = __builtin_amdgcn_readlane(wave_scan_add(n), 63);
+    return min(max((total + a.unit_target - 1) / a.unit_target, a.unit_tiles), kUnitTiles);
+}
+__device__ __forceinline__ PagedUnit paged_unit(const AttnArgs& a, int unit, int lane) {
+    if (a.unit_tiles == 0) {
+        const int len = __builtin_amdgcn_readfirstlane(a.lens[unit]);
+        return PagedUnit{unit, len, 0, paged_tiles(a, len)};
+    }
+    const int chunk = paged_chunk(a, lane);
+    int base = 0;
+    for (int i0 = 0; i0 < a.B; i0 += 64) {
+        const int len = i0 + lane < a.B ? a.lens[i0 + lane] : 0;
+        const int tiles = paged_tiles(a, len), n = (tiles + chunk - 1) / chunk;
+        const int incl = wave_scan_add(n), last = __builtin_amdgcn_readlane(incl, 63);
+        if (unit - base < last) {
+            const int at = __builtin_ctzll(__ballot(incl > unit - base));
+            const int mine = __builtin_amdgcn_readlane(tiles, at), count = __builtin_amdgcn_readlane(n, at);
+            const int split = unit - base - (__builtin_amdgcn_readlane(incl, at) - count);
+            const int per = (mine + count - 1) / count;
+            return PagedUnit{i0 + at, __builtin_amdgcn_readlane(len, at), split * per, min(per, mine - split * per)};
+        }
+        base += last;
+    }
+    return PagedUnit{-1, 0, 0, 0};
+}
+// The first unit of sequence b, and how many it has
+struct PagedUnits {
+    int first, count;
+};
+__device__ __forceinline__ PagedUnits paged_units(const AttnArgs& a, int b, int lane) {
+    const int chunk = paged_chunk(a, lane);
+    int base = 0;
+    for (int i0 = 0;; i0 += 64) {
+        const int tiles = i0 + lane < a.B ? paged_tiles(a, a.lens[i0 + lane]) : 0, n = (tiles + chunk - 1) / chunk;
+        const int incl = wave_scan_add(n);
+        if (b < i0 + 64) {
+            const int count = __builtin_amdgcn_readlane(n, b - i0);
+            return PagedUnits{base + __builtin_amdgcn_readlane(incl, b - i0) - count, count};
+        }
+        base += __builtin_amdgcn_readlane(incl, 63);
+    }
+}
 
 // Packs per row of the stored popcounts: S rounded up to 16, so that every
 // row starts 16-byte aligned and eight-key runs load whole.
@@ -79,9 +167,22 @@ bool mfma_split_ok(int D, int64_t chunk, int64_t head_groups);
 // Head dims whose kernels append a token in place (the one-slice row encoder
 // of encode_row.h takes power-of-two lane groups).
 __host__ __device__ constexpr bool append_dim(int D) { return D == 64 || D == 128 || D == 256; }
+// The paged instances (binary and compensated modes): grid.x units, grid.y kv
+// heads times query-head groups of a kv head; the partial of unit u and query
+// head h goes to ws[(u * Hq + h) * (D + 2)], or the outputs to a.out (one unit per
+// sequence).
+template <int D>
+void paged_launch(int mode, int G, const AttnArgs& a, dim3 grid, hipStream_t st);
+template <int D>
+int paged_occupancy(int mode, int G);
+bool launch_paged_split(int mode, int D, int G, const AttnArgs& a, dim3 grid, hipStream_t st);
+int paged_wgs_per_cu(int mode, int D, int G);
 // Resident workgroups per CU of the MFMA kernel of (mode, D, G) on the current
 // device (0 when no MFMA kernel handles it).
 int mfma_wgs_per_cu(int mode, int D, int G);
+
+// Query heads that one workgroup attends for, of the `group` that share a kv head.
+int attention_group(int group, int D, int mode);
 
 // New K/V token encoded into cache position `slot` by the attention launch
 // itself (see AttnArgs::app_k).

@@ -252,7 +252,8 @@ __device__ __forceinline__ void lds_barrier() {
 // tile's too (2048 MHA heads of 200 keys at d = 256: binary 20.4 us with a call,
 // 16.5 inlined, compensated 49.6 and 43.4).
 template <int D, int G, bool KMF, bool RES, int NT, int NQ>
-__device__ __forceinline__ void prep_digits(const uint16_t (&qpre)[NQ], QDigits<D, G, KMF>& qd, float* qf) {
+__device__ __forceinline__ void prep_digits(const uint16_t (&qpre)[NQ], QDigits<D, G, KMF>& qd, float* qf,
+                                            bool bf16 = false) {
     const int tid = threadIdx.x, lane = tid & 63;
     uint32_t* signs = &qd.signs[0][0];   // [G * D / 32] words, bit b of word i = element 32i + b
     __shared__ float gmax[G * D / 32];   // max |q| of each 32-element group (one head's)
@@ -265,7 +266,7 @@ __device__ __forceinline__ void prep_digits(const uint16_t (&qpre)[NQ], QDigits<
     for (int j = 0; j < NQ; j++) {
         const int i = tid + NT * j;
         if (i - lane >= G * D) break;   // (uniform)
-        const float x = h2f(qpre[j]);
+        const float x = bf16 ? __builtin_bit_cast(float, (uint32_t)qpre[j] << 16) : h2f(qpre[j]);
         const uint64_t bits = __ballot(x >= 0.0f);
         const float wm = half_max(fabsf(x));
         if (i < G * D) {
@@ -471,6 +472,10 @@ __host__ __device__ constexpr bool k_on_mfma(int G, int mode) {
 // w + 2 NW, ... of the key range, and the epilogue merges the NW waves.
 // APP: the workgroup whose key range holds the slot a.app_slot appends the
 // token a.app_k / a.app_v there.
+// PG: a paged cache (kv_rows pages times kv heads, kv_stride the page size): the
+// workgroup takes work unit blockIdx.x (PagedUnit) of kv head and group
+// blockIdx.y; a tile lies in one page, so each tile's loads go through buffer
+// resources of its own, over its keys alone.
 //
 // The scalar arguments (14 dwords) come in registers with the wave (kernarg
 // preloading: a launch's first read of its argument memory takes about a
@@ -488,7 +493,10 @@ inline int pack_plan(const AttnArgs& a, int G) {
 #define BC_MFMA_ARGS(a, G)                                                                       \
     (a).q, (a).kb.signs, (a).vb.signs, (a).kr.codes, (a).vr.codes, (a).B * (a).Hkv, (a).S,       \
         (a).kv_stride, pack_plan(a, G), (a)
-template <int D, int G, int MODE, int NW = 4, bool APP = false>
+#define BC_PAGED_ARGS(a, G)                                                                      \
+    (a).q, (a).kb.signs, (a).vb.signs, (a).kr.codes, (a).vr.codes, (a).n_pages * (a).Hkv, 0,     \
+        (a).page_tiles * 64, ((a).Hq / (a).Hkv / (G)) << kPlanGroups, (a)
+template <int D, int G, int MODE, int NW = 4, bool APP = false, bool PG = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(Occupancy<D, G, MODE>::kWaves)))
 void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* v_signs,
                       const uint8_t* k_codes, const uint8_t* v_codes, int kv_rows, int S, int kv_stride,
@@ -574,6 +582,7 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
     __shared__ float wm[NW][G], wlsum[NW][G], wsc[NW][G];
     // (groups of eight) the merge's factors per head: each wave's, maximum, total
     __shared__ float wfac[G == 8 ? NW : 1][G], wtot[G == 8 ? 2 : 1][G];
+    __shared__ int wbad[PG ? NW : 1];   // (paged) the wave met a page outside the pool
 
     const int split = blockIdx.x;
     // per-head modes: this launch's query-head groups come from its list
@@ -586,6 +595,12 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
     }
     // groups are numbered through batches, kv heads and the groups of a kv head
     const int nqg = plan >> kPlanGroups;
+    bc::PagedUnit unit{0, 0, 0, 0};
+    if constexpr (PG) {
+        unit = bc::paged_unit(a, split, threadIdx.x & 63);
+        if (unit.b < 0) return;
+        grow += unit.b * a.Hkv * nqg;
+    }
     const int bkv = grow / nqg;
     const int bhq0 = grow * G;   // first query head
     const int64_t cap = (int64_t)kv_rows * kv_stride;
@@ -594,10 +609,23 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
     // loop in scalar registers (a uniform loop, not an exec-masked one)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int g4 = lane >> 4, lj = lane & 15;
-    const int chunk = (plan & (kPlanList - 1)) * 64;
-    const int key_begin = split * chunk;
-    const int key_end = min(S, key_begin + chunk);
-    const int64_t kv_base = (int64_t)bkv * kv_stride;
+    const int chunk = PG ? unit.tiles * 64 : (plan & (kPlanList - 1)) * 64;
+    const int key_begin = PG ? a.key0 + unit.first * 64 : split * chunk;
+    const int key_end = min(PG && unit.tiles > 0 ? unit.len : S, key_begin + chunk);
+    const int64_t kv_base = PG ? 0 : (int64_t)bkv * kv_stride;
+    // (paged) where the wave's i-th tile lies, in lane i: its first vector / 64
+    // within the planes; tiles of pages outside the pool read the pool's first
+    int tile_at = 0;
+    bool bad_page = false;
+    if constexpr (PG) {
+        const int ti = wave + NW * lane;
+        if (ti < unit.tiles) {
+            const int tile = key_begin / 64 + ti;
+            const int page = a.tables[(int64_t)unit.b * a.width + tile / a.page_tiles];
+            bad_page = page < 0 || page >= a.n_pages;
+            tile_at = ((bad_page ? 0 : page) * a.Hkv + (bkv - unit.b * a.Hkv)) * a.page_tiles + tile % a.page_tiles;
+        }
+    }
     const float isd2 = (1.0f / sqrtf((float)D)) * kLog2e;
     const int kown = lane;   // the key whose score this lane computes (tile-relative)
     // V code tiles of compensated mode (linear rows of CB bytes): the 16-byte
@@ -617,6 +645,17 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
         return __builtin_amdgcn_make_buffer_rsrc(
             (void*)((const uint8_t*)plane + (kv_base + key_begin) * rb), (short)0, nk * rb, kBufWord3);
     };
+    // the resource of tile t0's loads: the range's, or (paged) the tile's own
+    auto at_tile = [&](const __amdgpu_buffer_rsrc_t& whole, const void* plane, int rb, int t0) {
+        if constexpr (PG) {
+            const int keys = min(max(key_end - t0, 0), 64);
+            const int i = (t0 - key_begin) / (64 * NW) & 63;   // (past the range: any tile, no keys)
+            const int64_t v = (int64_t)(uint32_t)__builtin_amdgcn_readlane(tile_at, i) * 64;
+            return __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)plane + v * rb), (short)0, keys * rb, kBufWord3);
+        } else {
+            return whole;
+        }
+    };
     const __amdgpu_buffer_rsrc_t r_ks = rsrc(k_signs, SB), r_vs = rsrc(v_signs, SB);
     const __amdgpu_buffer_rsrc_t r_ksc = rsrc(k_signs + cap * SB, 2), r_vsc = rsrc(v_signs + cap * SB, 2);
     const __amdgpu_buffer_rsrc_t r_kc = rsrc(k_codes, CB), r_vc = rsrc(v_codes, CB);
@@ -634,11 +673,12 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
     // ---------------- loads of one tile: K side into registers, V side to LDS
     // the lane's code pieces of key block kb (KBlocks), its key's row at byte
     // offset row (kOob: zeros)
-    auto load_kblock = [&](KR& r, int kb, int row) {
+    auto load_kblock = [&](KR& r, int kb, int row, int t0) {
         constexpr int aux = MODE == MODE_ADAPTIVE ? 0 : BC_NT_AUX;
+        const __amdgpu_buffer_rsrc_t r_kct = at_tile(r_kc, k_codes, CB, t0);
 #pragma unroll
         for (int pc = 0; pc < KB::kPieces; pc++) {
-            const v4u_t c = __builtin_amdgcn_raw_buffer_load_b128(r_kc, row + 64 * pc + 16 * g4, 0, aux);
+            const v4u_t c = __builtin_amdgcn_raw_buffer_load_b128(r_kct, row + 64 * pc + 16 * g4, 0, aux);
             const int i = kb * KB::kWords + 4 * pc;
             r.kc[i] = c[0]; r.kc[i + 1] = c[1]; r.kc[i + 2] = c[2]; r.kc[i + 3] = c[3];
         }
@@ -647,13 +687,13 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
             // (a lane group past the row's units repeats the unit two back)
             constexpr int left = KB::kLeft;
             const int q = 4 * tl + 2 < left ? g4 : (g4 & 1);
-            const v2u_t c = __builtin_amdgcn_raw_buffer_load_b64(r_kc, row + 64 * KB::kPieces + 32 * tl + 8 * q, 0, aux);
+            const v2u_t c = __builtin_amdgcn_raw_buffer_load_b64(r_kct, row + 64 * KB::kPieces + 32 * tl + 8 * q, 0, aux);
             const int i = kb * KB::kWords + 4 * KB::kPieces + 2 * tl;
             r.kc[i] = c[0]; r.kc[i + 1] = c[1];
         }
     };
     auto load_k = [&](KR& r, int t0) {
-        const int tr = t0 - key_begin;      // tile offset in the range (keys)
+        const int tr = PG ? 0 : t0 - key_begin;      // tile offset in the range (keys)
         const int kk = tr + kown;
         if constexpr (MODE == MODE_ADAPTIVE) {
             // popcounts and the two binary scales; residual data is gathered
@@ -677,28 +717,29 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
             r.rsv = 0;
             return;
         }
-        r.ks = buf_signs<D, BC_NT_AUX>(r_ks, kk * SB);
-        r.sk = __builtin_amdgcn_raw_buffer_load_b16(r_ksc, kk * 2, 0, BC_NT_SCALES);
-        r.svv = __builtin_amdgcn_raw_buffer_load_b16(r_vsc, kk * 2, 0, BC_NT_SCALES);
+        r.ks = buf_signs<D, BC_NT_AUX>(at_tile(r_ks, k_signs, SB, t0), kk * SB);
+        r.sk = __builtin_amdgcn_raw_buffer_load_b16(at_tile(r_ksc, k_signs + cap * SB, 2, t0), kk * 2, 0, BC_NT_SCALES);
+        r.svv = __builtin_amdgcn_raw_buffer_load_b16(at_tile(r_vsc, v_signs + cap * SB, 2, t0), kk * 2, 0, BC_NT_SCALES);
         r.rsk = 0;
         r.rsv = 0;
         // residual scales and K codes of every key (adaptive mode too: the
         // selection is known only after the scores, and these loads are the
         // ones worth prefetching; V codes are gathered for selected keys)
         if constexpr (RES) {
-            r.rsk = __builtin_amdgcn_raw_buffer_load_b16(r_krs, kk * 2, 0, BC_NT_SCALES);
-            r.rsv = __builtin_amdgcn_raw_buffer_load_b16(r_vrs, kk * 2, 0, BC_NT_SCALES);
+            r.rsk = __builtin_amdgcn_raw_buffer_load_b16(at_tile(r_krs, k_codes + cap * CB, 2, t0), kk * 2, 0, BC_NT_SCALES);
+            r.rsv = __builtin_amdgcn_raw_buffer_load_b16(at_tile(r_vrs, v_codes + cap * CB, 2, t0), kk * 2, 0, BC_NT_SCALES);
             if constexpr (KMF) {
                 // key block kb: key 16kb + l%16
 #pragma unroll
-                for (int kb = 0; kb < 4; kb++) load_kblock(r, kb, (tr + 16 * kb + lj) * CB);
+                for (int kb = 0; kb < 4; kb++) load_kblock(r, kb, (tr + 16 * kb + lj) * CB, t0);
             }
         }
     };
     // V tile to LDS: key k's sign row at k*SB; its code row at k*CB (linear,
     // pieces swizzled as above) or piece c at c*1024 + 16k (per key)
     auto issue_v = [&](int buf, int t0) {
-        const int tr = t0 - key_begin;
+        const int tr = PG ? 0 : t0 - key_begin;
+        const __amdgpu_buffer_rsrc_t r_vst = at_tile(r_vs, v_signs, SB, t0);
         uint8_t* st_codes = buf ? lds_st1[wave] : lds_st0[wave];
         uint8_t* st_signs = st_codes + WL::kCodeBytes;
         if constexpr (WL::kSignPad) {
@@ -707,24 +748,25 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
             const int w = min(lane % RW, SB / 4 - 1);
 #pragma unroll
             for (int c = 0; c < RW; c++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vs, LDS_PTR(void, st_signs + c * 256), 4,
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vst, LDS_PTR(void, st_signs + c * 256), 4,
                                                          (tr + c * (64 / RW) + lane / RW) * SB + 4 * w, 0, 0, 0);
         } else {
             // whole KiB, and a half one at d = 64 and 192 (whose lanes 32..63
             // repeat lanes 0..31 into the half past the rows)
 #pragma unroll
             for (int c = 0; c < SB / 16; c++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vs, LDS_PTR(void, st_signs + c * 1024), 16,
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vst, LDS_PTR(void, st_signs + c * 1024), 16,
                                                          tr * SB + 16 * lane + c * 1024, 0, 0, BC_NT_AUX);
             if constexpr (SB % 16 != 0)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vs, LDS_PTR(void, st_signs + SB / 16 * 1024), 16,
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vst, LDS_PTR(void, st_signs + SB / 16 * 1024), 16,
                                                          tr * SB + 16 * (lane & 31) + SB / 16 * 1024, 0, 0, 0);
         }
         if constexpr (ALLRES) {
+            const __amdgpu_buffer_rsrc_t r_vct = at_tile(r_vc, v_codes, CB, t0);
 #pragma unroll
             for (int c = 0; c < Q; c++)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    r_vc, LDS_PTR(void, st_codes + c * 1024), 16,
+                    r_vct, LDS_PTR(void, st_codes + c * 1024), 16,
                     LIN_V ? tr * CB + c * 1024 + 16 * (Q_POW2 ? lane ^ ((4 * c + (lane >> 4)) & (Q - 1)) : lane)
                           : (tr + lane) * CB + 16 * c, 0, 0, LIN_V ? BC_NT_AUX : 0);
         }
@@ -767,7 +809,8 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
         app_raw = bc::load_row_slice((lane / AL == 1 ? a.app_v : a.app_k) + (int64_t)bkv * D, lane % AL);
         __builtin_amdgcn_sched_barrier(0);
     }
-    prep_digits<D, G, KMF, RES, NT>(qpre, qd, qf);
+    if constexpr (PG) prep_digits<D, G, KMF, RES, NT>(qpre, qd, qf, a.bf16 != 0);
+    else prep_digits<D, G, KMF, RES, NT>(qpre, qd, qf);
 
     // In-place append: the wave that takes the slot's tile encodes the token's
     // K and V vectors (online-encode semantics: the residual against the fp32
@@ -1098,7 +1141,7 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
             for (int kb = 0; kb < 4; kb++) {
                 const int j = 16 * kb + lj;
                 const int key = __builtin_amdgcn_ds_bpermute(4 * j, key_at);
-                load_kblock(r, kb, j < nsel ? (tr + key) * CB : kOob);
+                load_kblock(r, kb, j < nsel ? (tr + key) * CB : kOob, t0);
             }
         } else {
 #pragma unroll
@@ -1784,6 +1827,10 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
             wsc[wave][g] = I8 ? pow2_inv(es[g]) : ldexpf(1.0f, -wexp);
         }
     }
+    if constexpr (PG) {
+        const bool bad = __ballot(bad_page) != 0ull || bc::paged_bad_len(a, unit.len);
+        if (lane == 0) wbad[wave] = bad;
+    }
     // groups of eight form the merge's factors once per head (one barrier more;
     // the first below publishes them), not for each of its elements: binary 64
     // groups of 200 keys, d = 256, 15.7 -> 14.5 us, compensated 21.2 -> 20.4
@@ -1918,7 +1965,23 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
                     if (live) L += f * wlsum[w][g];
                 }
             }
-            if (a.out != nullptr) {
+            if constexpr (PG) {
+                bool bad = false;
+#pragma unroll
+                for (int w = 0; w < NW; w++) bad |= wbad[w] != 0;
+                if (a.out != nullptr) {
+                    // one unit per sequence: the output itself
+                    const float o = bad ? __builtin_nanf("") : L == 0.0f ? 0.0f : accv * (1.0f / L);
+                    a.out[(int64_t)(bhq0 + g) * D + e] = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o) : f2h(o);
+                } else {
+                    float* dst = a.ws + ((int64_t)split * a.Hq + (bhq0 + g - unit.b * a.Hq)) * (D + 2);
+                    dst[2 + e] = accv;
+                    if (e == 0) {
+                        dst[0] = M;
+                        dst[1] = bad ? __builtin_nanf("") : L;
+                    }
+                }
+            } else if (a.out != nullptr) {
                 // one split: the output itself, normalised as the merge of a
                 // single partial would (factor 1, sum l)
                 a.out[(int64_t)(bhq0 + g) * D + e] = f2h(L > 0.0f ? accv * (1.0f / L) : 0.0f);
@@ -1970,6 +2033,24 @@ void launch_dg(int mode, const AttnArgs& a, dim3 grid, hipStream_t st) {
 }
 
 template <int D, int G>
+void launch_paged_dg(int mode, const AttnArgs& a, dim3 grid, hipStream_t st) {
+    if (mode == MODE_BINARY)
+        hipLaunchKernelGGL((attn_mfma_kernel<D, G, MODE_BINARY, 4, false, true>), grid, dim3(256), 0, st, BC_PAGED_ARGS(a, G));
+    else
+        hipLaunchKernelGGL((attn_mfma_kernel<D, G, MODE_COMP, 4, false, true>), grid, dim3(256), 0, st, BC_PAGED_ARGS(a, G));
+}
+
+template <int D, int G>
+int occupancy_paged_dg(int mode) {
+    int n = 0;
+    void (*kernel)(const uint16_t*, const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, int, int, int, int,
+                   AttnArgs) = attn_mfma_kernel<D, G, MODE_BINARY, 4, false, true>;
+    if (mode != MODE_BINARY) kernel = attn_mfma_kernel<D, G, MODE_COMP, 4, false, true>;
+    const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, 0);
+    return e == hipSuccess ? n : 0;
+}
+
+template <int D, int G>
 int occupancy_dg(int mode) {
     int n = 0;
     hipError_t e;
@@ -1999,6 +2080,26 @@ bool mfma_launch(int mode, int G, const AttnArgs& a, dim3 grid, hipStream_t st, 
         default: launch_dg<D, 1>(mode, a, grid, st); break;
     }
     return true;
+}
+
+template <int D>
+void paged_launch(int mode, int G, const AttnArgs& a, dim3 grid, hipStream_t st) {
+    switch (G) {
+        case 8: launch_paged_dg<D, 8>(mode, a, grid, st); break;
+        case 4: launch_paged_dg<D, 4>(mode, a, grid, st); break;
+        case 2: launch_paged_dg<D, 2>(mode, a, grid, st); break;
+        default: launch_paged_dg<D, 1>(mode, a, grid, st); break;
+    }
+}
+
+template <int D>
+int paged_occupancy(int mode, int G) {
+    switch (G) {
+        case 8: return occupancy_paged_dg<D, 8>(mode);
+        case 4: return occupancy_paged_dg<D, 4>(mode);
+        case 2: return occupancy_paged_dg<D, 2>(mode);
+        default: return occupancy_paged_dg<D, 1>(mode);
+    }
 }
 
 template <int D>

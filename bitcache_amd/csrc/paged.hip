@@ -1,134 +1,97 @@
-// Decode attention over a paged compressed cache, a length per sequence.
-//
-// Simple form: a workgroup per (sequence, query head), its four waves take
-// 64-key tiles in turn.  Scores: lane = key.  Values: lane = dimension, one key
-// after the other.  Online softmax per wave, merged over the waves at the end.
+// Decode attention over a paged compressed cache, a length per sequence: host side
+// and merge.  The attention itself is attn_mfma_kernel.h's paged instances over
+// work units that the device cuts from the lengths (attn.h, PagedUnit).
 #include <math.h>
 
 #include "attn.h"
 
 namespace {
-using bc::kLog2e;
+using bc::AttnArgs;
+using bc::MODE_BINARY;
+using bc::MODE_COMP;
 
-struct PagedArgs {
-    const uint16_t* q;
-    BinPlanes kb, vb;
-    ResPlanes kr, vr;
-    const int32_t* tables;
-    const int32_t* lens;
-    uint16_t* out;
-    int Hq, Hkv, n_pages, page_size, width, max_len;
+// The merge of a sequence's units: one workgroup per (sequence, query head), the
+// partials spread over its 256 / D groups of threads (one of at least D).
+template <int D>
+__global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t* out) {
+    constexpr int P = 256 / D;
+    __shared__ float fac[256];
+    __shared__ float red[P * D];
+    __shared__ float wmax[4], wsum[4];
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bc::PagedUnits u = bc::paged_units(a, b, lane);
+    const float* p0 = a.ws + ((int64_t)u.first * a.Hq + h) * (D + 2);
+    const int64_t step = (int64_t)a.Hq * (D + 2);
+    const int part = tid / D, e = tid % D;
+    // online over blocks of 256 partials
+    float M = -INFINITY, L = 0.0f, acc = 0.0f;
+    for (int s0 = 0; s0 < u.count; s0 += 256) {
+        const int n = min(256, u.count - s0);
+        const float* p = p0 + s0 * step;
+        const float m = tid < n ? p[tid * step] : -INFINITY;
+        const float l = tid < n ? p[tid * step + 1] : 0.0f;
+        const float mw = wave_max(m);
+        if (lane == 0) wmax[wave] = mw;
+        __syncthreads();
+        const float mn = fmaxf(fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3])), M);
+        const float f = m == -INFINITY ? 0.0f : exp2f(m - mn);
+        fac[tid] = f;
+        // (a NaN sum marks a bad page: it stays one at any factor)
+        const float lw = wave_sum(l == l ? f * l : l);
+        if (lane == 0) wsum[wave] = lw;
+        __syncthreads();
+        const float old = M == -INFINITY ? 0.0f : exp2f(M - mn);
+        L = L * old + ((wsum[0] + wsum[1]) + (wsum[2] + wsum[3]));
+        acc *= old;
+        if (part < P) {
+#pragma unroll 8
+            for (int s = part; s < n; s += P) acc += fac[s] * p[s * step + 2 + e];
+        }
+        M = mn;
+        __syncthreads();
+    }
+    if (part < P) red[part * D + e] = acc;
+    __syncthreads();
+    if (tid < D) {
+        float o = red[tid];
+#pragma unroll
+        for (int q = 1; q < P; q++) o += red[q * D + tid];
+        // (NaN where the length is out of bounds)
+        o = bc::paged_bad_len(a, a.lens[b]) ? __builtin_nanf("") : L == 0.0f ? 0.0f : o * (1.0f / L);
+        out[((int64_t)b * a.Hq + h) * D + tid] = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o) : f2h(o);
+    }
+}
+
+struct PagedPlan {
+    int G, groups;     // query heads of a workgroup, workgroups per sequence and unit
+    int unit_tiles, unit_target;
+    int units;         // at most
+    size_t bytes;      // of partials
 };
 
-template <bool BF>
-__device__ __forceinline__ float q_f(uint16_t h) {
-    if constexpr (BF) return __builtin_bit_cast(float, (uint32_t)h << 16);
-    return h2f(h);
-}
-
-__device__ __forceinline__ float nibble(uint32_t w, int i) { return (float)((int)(w << (28 - 4 * i)) >> 28); }
-
-template <int D, bool BF, bool RES>
-__global__ __launch_bounds__(256) void paged_kernel(PagedArgs a) {
-    constexpr int N = (D + 63) / 64;
-    __shared__ float qf[D];
-    __shared__ uint32_t qs[D / 32];
-    __shared__ float acc_w[4][D], m_w[4], l_w[4];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int hkv = h / (a.Hq / a.Hkv);
-    const int64_t row = (int64_t)b * a.Hq + h;
-    const int len = a.lens[b];
-    const bool bad_len = len > a.max_len || (int64_t)len > (int64_t)a.width * a.page_size;
-    if (tid < D) qf[tid] = q_f<BF>(a.q[row * D + tid]);
-    __syncthreads();
-    if (tid < D / 32) {
-        uint32_t w = 0;
-        for (int i = 0; i < 32; i++) w |= (qf[32 * tid + i] >= 0.0f ? 1u : 0u) << i;
-        qs[tid] = w;
+PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len, int d) {
+    PagedPlan p{};
+    p.G = bc::attention_group(n_heads / n_kv_heads, d, mode);
+    p.groups = n_kv_heads * (n_heads / n_kv_heads / p.G);
+    const int64_t tiles = ((int64_t)max_seq_len + 63) / 64;
+    const int cu = bc::device_cu_count();
+    int fit = bc::paged_wgs_per_cu(mode, d, p.G);
+    if (fit <= 0) fit = 3;
+    p.unit_target = (int)((2LL * fit * cu + p.groups - 1) / p.groups);
+    // (at least two tiles a wave, one where that leaves CUs idle)
+    p.unit_tiles = (int64_t)batch * p.groups * ((tiles + 7) / 8) < cu ? 4 : 8;
+    if (tiles <= p.unit_tiles) {
+        p.unit_tiles = 0;
+        p.units = batch;
+        return p;
     }
-    float scale_q = 0.0f;
-    for (int i = 0; i < D; i++) scale_q += fabsf(qf[i]);
-    scale_q /= (float)D;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, acc[N];
-    for (int n = 0; n < N; n++) acc[n] = 0.0f;
-    bool bad = bad_len;
-    for (int t0 = wave * 64; t0 < len && !bad; t0 += 256) {
-        const int page = a.tables[(int64_t)b * a.width + t0 / a.page_size];
-        if (page < 0 || page >= a.n_pages) {
-            bad = true;
-            break;
-        }
-        const int64_t v0 = ((int64_t)page * a.Hkv + hkv) * a.page_size + t0 % a.page_size;
-        const int n_keys = min(64, len - t0);
-        float sc = -INFINITY;
-        if (lane < n_keys) {
-            const int64_t v = v0 + lane;
-            int pc = 0;
-            for (int w = 0; w < D / 32; w++) pc += __builtin_popcount(~(qs[w] ^ ((const uint32_t*)(a.kb.signs + v * (D / 8)))[w]));
-            float s = scale_q * h2f(a.kb.scales[v]) * (float)(2 * pc - D);
-            if constexpr (RES) {
-                float r = 0.0f;
-                for (int w = 0; w < D / 8; w++) {
-                    const uint32_t c = ((const uint32_t*)(a.kr.codes + v * (D / 2)))[w];
-                    for (int i = 0; i < 8; i++) r = fmaf(qf[8 * w + i], nibble(c, i), r);
-                }
-                s = fmaf(r, h2f(a.kr.scales[v]) * (1.0f / 7.0f), s);
-            }
-            sc = s * ((1.0f / sqrtf((float)D)) * kLog2e);
-        }
-        const float mn = fmaxf(m, wave_max(sc));
-        const float f = m == -INFINITY ? 0.0f : exp2f(m - mn);
-        const float p = lane < n_keys ? exp2f(sc - mn) : 0.0f;
-        l = l * f + p;
-        for (int n = 0; n < N; n++) acc[n] *= f;
-        m = mn;
-        for (int k = 0; k < n_keys; k++) {
-            const float pk = __shfl(p, k);
-            const int64_t v = v0 + k;
-            const float sv = h2f(a.vb.scales[v]);
-            float rv = 0.0f;
-            if constexpr (RES) rv = h2f(a.vr.scales[v]) * (1.0f / 7.0f);
-            for (int n = 0; n < N; n++) {
-                const int e = 64 * n + lane;
-                if (e >= D) continue;
-                float x = (a.vb.signs[v * (D / 8) + e / 8] >> (e % 8)) & 1 ? sv : -sv;
-                if constexpr (RES) x += rv * nibble(a.vr.codes[v * (D / 2) + e / 2], e & 1);
-                acc[n] = fmaf(pk, x, acc[n]);
-            }
-        }
-    }
-    for (int n = 0; n < N; n++)
-        if (64 * n + lane < D) acc_w[wave][64 * n + lane] = acc[n];
-    const float lw = wave_sum(l);
-    if (lane == 0) {
-        m_w[wave] = m;
-        l_w[wave] = bad ? __builtin_nanf("") : lw;
-    }
-    __syncthreads();
-    for (int e = tid; e < D; e += 256) {
-        float M = -INFINITY, L = 0.0f, x = 0.0f;
-        for (int w = 0; w < 4; w++) M = fmaxf(M, m_w[w]);
-        for (int w = 0; w < 4; w++) {
-            if (l_w[w] != l_w[w]) L = x = l_w[w];
-            if (m_w[w] == -INFINITY) continue;
-            const float f = exp2f(m_w[w] - M);
-            L += f * l_w[w];
-            x += f * acc_w[w][e];
-        }
-        const float o = L == 0.0f ? 0.0f : x / L;
-        if constexpr (BF) a.out[row * D + e] = __builtin_bit_cast(uint16_t, (__bf16)o);
-        else a.out[row * D + e] = f2h(o);
-    }
-}
-
-template <int D>
-void launch(const PagedArgs& a, int batch, bool bf, bool res, hipStream_t st) {
-    const dim3 grid(a.Hq, batch);
-    if (bf && res) hipLaunchKernelGGL((paged_kernel<D, true, true>), grid, dim3(256), 0, st, a);
-    else if (bf) hipLaunchKernelGGL((paged_kernel<D, true, false>), grid, dim3(256), 0, st, a);
-    else if (res) hipLaunchKernelGGL((paged_kernel<D, false, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_kernel<D, false, false>), grid, dim3(256), 0, st, a);
+    const int64_t most = (int64_t)batch * ((tiles + p.unit_tiles - 1) / p.unit_tiles);
+    const int64_t capped = ((int64_t)batch * tiles + bc::kUnitTiles - 1) / bc::kUnitTiles;
+    int64_t units = (capped > p.unit_target ? capped : p.unit_target) + batch;
+    if (units > most) units = most;
+    p.units = (int)units;
+    p.bytes = (size_t)units * n_heads * (d + 2) * sizeof(float);
+    return p;
 }
 
 int validate(int batch, int n_heads, int n_kv_heads, int max_seq_len, int shared_len, int d) {
@@ -142,6 +105,9 @@ int validate(int batch, int n_heads, int n_kv_heads, int max_seq_len, int shared
     BC_REQUIRE(shared_len <= max_seq_len, BC_ERR_INVALID_ARGUMENT, "shared_len (%d) above max_seq_len (%d)",
                shared_len, max_seq_len);
     BC_REQUIRE(batch <= 65535, BC_ERR_UNSUPPORTED, "batch above 65535");
+    BC_REQUIRE(n_heads <= 65535, BC_ERR_UNSUPPORTED, "n_heads above 65535");
+    BC_REQUIRE((int64_t)batch * (max_seq_len / 64 + 1) <= INT32_MAX, BC_ERR_UNSUPPORTED,
+               "batch * max_seq_len above 2^37");
     return BC_OK;
 }
 
@@ -153,6 +119,11 @@ extern "C" int bc_paged_attention_workspace_size(int batch, int n_heads, int n_k
     const int rc = validate(batch, n_heads, n_kv_heads, max_seq_len, shared_len, head_dim);
     if (rc != BC_OK) return rc;
     *bytes = 0;
+    if ((int64_t)batch * n_heads == 0) return BC_OK;
+    for (int mode : {MODE_BINARY, MODE_COMP}) {
+        const size_t n = plan(mode, batch, n_heads, n_kv_heads, max_seq_len, head_dim).bytes;
+        if (n > *bytes) *bytes = n;
+    }
     return BC_OK;
 }
 
@@ -167,6 +138,9 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     BC_REQUIRE(n_pages >= 0 && page_size > 0 && page_size % 64 == 0, BC_ERR_INVALID_ARGUMENT,
                "page_size must be a multiple of 64, got %d (n_pages %d)", page_size, n_pages);
     BC_REQUIRE((int64_t)n_pages * page_size <= INT32_MAX, BC_ERR_UNSUPPORTED, "more than 2^31 - 1 slots");
+    // (a tile's place among the pool's tiles is an int)
+    BC_REQUIRE((int64_t)n_pages * (page_size / 64) * n_kv_heads <= INT32_MAX, BC_ERR_UNSUPPORTED,
+               "more than 2^37 vectors in the pool");
     BC_REQUIRE(table_width >= 0, BC_ERR_INVALID_ARGUMENT, "negative table width");
     BC_REQUIRE(shared_len % page_size == 0 && shared_len / page_size <= table_width, BC_ERR_INVALID_ARGUMENT,
                "shared_len (%d) must be whole pages of %d slots within the tables", shared_len, page_size);
@@ -175,29 +149,44 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     if ((int64_t)batch * n_heads == 0) return BC_OK;
     BC_REQUIRE(q && out && seq_lens && (table_width == 0 || block_tables) && (n_pages == 0 || (k_bin && v_bin)),
                BC_ERR_INVALID_ARGUMENT, "null pointer");
+    const int mode = k_res ? MODE_COMP : MODE_BINARY;
+    const PagedPlan p = plan(mode, batch, n_heads, n_kv_heads, max_seq_len, head_dim);
+    BC_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes), BC_ERR_WORKSPACE,
+               "workspace of %zu bytes required, got %zu", p.bytes, workspace_bytes);
+    BC_REQUIRE(p.groups <= 65535, BC_ERR_UNSUPPORTED, "more than 65535 head groups");
     const int64_t cap = (int64_t)n_pages * n_kv_heads * page_size;
-    PagedArgs a{};
+    hipStream_t st = (hipStream_t)stream;
+    AttnArgs a{};
     a.q = (const uint16_t*)q;
     a.kb = bin_planes(k_bin, cap, head_dim);
     a.vb = bin_planes(v_bin, cap, head_dim);
     if (k_res) a.kr = res_planes(k_res, cap, head_dim);
     if (v_res) a.vr = res_planes(v_res, cap, head_dim);
-    a.tables = block_tables;
-    a.lens = seq_lens;
-    a.out = (uint16_t*)out;
+    a.B = batch;
     a.Hq = n_heads;
     a.Hkv = n_kv_heads;
-    a.n_pages = n_pages;
-    a.page_size = page_size;
+    a.ws = (float*)workspace;
+    a.lens = seq_lens;
+    a.tables = block_tables;
     a.width = table_width;
-    a.max_len = max_seq_len;
-    const bool bf = dtype == BC_BF16, res = k_res != nullptr;
-    hipStream_t st = (hipStream_t)stream;
+    a.n_pages = n_pages;
+    a.page_tiles = page_size / 64;
+    a.max_len = n_pages > 0 ? max_seq_len : 0;   // (without pages no length but zero is right)
+    a.unit_tiles = p.unit_tiles;
+    a.unit_target = p.unit_target;
+    a.bf16 = dtype == BC_BF16;
+    if (p.unit_tiles == 0) a.out = (uint16_t*)out;
+    BC_REQUIRE(bc::launch_paged_split(mode, head_dim, p.G, a, dim3(p.units, p.groups), st), BC_ERR_UNSUPPORTED,
+               "head_dim %d", head_dim);
+    const int launched = bc::check_launch("paged attention");
+    if (launched != BC_OK || p.unit_tiles == 0) return launched;
+    const dim3 grid(n_heads, batch);
     switch (head_dim) {
-#define BC_CASE(DD) case DD: launch<DD>(a, batch, bf, res, st); break;
+#define BC_CASE(DD) \
+    case DD: hipLaunchKernelGGL((paged_combine_kernel<DD>), grid, dim3(256), 0, st, a, (uint16_t*)out); break;
         BC_CASE(32) BC_CASE(64) BC_CASE(96) BC_CASE(128) BC_CASE(160) BC_CASE(192) BC_CASE(224) BC_CASE(256)
 #undef BC_CASE
         default: return bc::set_error(BC_ERR_UNSUPPORTED, "head_dim %d", head_dim);
     }
-    return bc::check_launch("paged attention");
+    return bc::check_launch("paged attention merge");
 }

@@ -61,8 +61,12 @@ __device__ __forceinline__ float to_f(uint16_t h) {
     if constexpr (BF) return __builtin_bit_cast(float, (uint32_t)h << 16);
     return h2f(h);
 }
+// (the empty asm: the compiler would join the roundings to 32 and to 16 bits into
+// a conversion from 64, some thirty instructions that give another value for
+// every 2^13th element)
 template <bool BF>
 __device__ __forceinline__ uint16_t from_f(float f) {
+    asm volatile("" : "+v"(f));
     if constexpr (BF) return __builtin_bit_cast(uint16_t, (__bf16)f);
     return f2h(f);
 }
