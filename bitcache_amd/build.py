@@ -29,7 +29,7 @@ EXT = os.path.join(HERE, "_C" + EXT_SUFFIX)
 
 # (the longest compiles first: the matrix-core attention kernels, one file per head dim)
 HIP_SOURCES = [f"attn_{kind}_d{d}.hip" for d in (256, 224, 192, 160, 128, 96, 64, 32)
-               for kind in ("mfma", "paged")] + [
+               for kind in ("mfma", "paged")] + [f"prefix_attn_d{d}.hip" for d in (256, 192, 128, 64)] + [
     "attention.hip", "adaptive.hip", "encode.hip", "rotary.hip", "paged.hip", "attention_mfma.hip", "convert.hip", "probe.hip", "abi.cpp"]
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",

@@ -4,32 +4,45 @@
 #include <math.h>
 
 #include "attn.h"
+#include "prefix_attn.h"
+
+namespace bc {
+extern template int prefix_launch<64>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+extern template int prefix_launch<128>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+extern template int prefix_launch<192>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+extern template int prefix_launch<256>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+}  // namespace bc
 
 namespace {
 using bc::AttnArgs;
+using bc::PrefixArgs;
 using bc::MODE_BINARY;
 using bc::MODE_COMP;
 
-// The merge of a sequence's units: one workgroup per (sequence, query head), the
+// The merge of a sequence's units, and of the shared prefix's splits (prefix:
+// `splits` partials per row): one workgroup per (sequence, query head), the
 // partials spread over its 256 / D groups of threads (one of at least D).
 template <int D>
-__global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t* out) {
+__global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t* out, const float* prefix, int splits) {
     constexpr int P = 256 / D;
     __shared__ float fac[256];
     __shared__ float red[P * D];
     __shared__ float wmax[4], wsum[4];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const bc::PagedUnits u = bc::paged_units(a, b, lane);
-    const float* p0 = a.ws + ((int64_t)u.first * a.Hq + h) * (D + 2);
-    const int64_t step = (int64_t)a.Hq * (D + 2);
+    const int64_t own_step = (int64_t)a.Hq * (D + 2), prefix_step = own_step * a.B;
+    const float* own = a.ws + (int64_t)u.first * own_step + (int64_t)h * (D + 2);
+    const float* shared = prefix + ((int64_t)b * a.Hq + h) * (D + 2);
+    const int total = splits + u.count;
+    auto partial = [&](int s) { return s < splits ? shared + s * prefix_step : own + (s - splits) * own_step; };
     const int part = tid / D, e = tid % D;
     // online over blocks of 256 partials
     float M = -INFINITY, L = 0.0f, acc = 0.0f;
-    for (int s0 = 0; s0 < u.count; s0 += 256) {
-        const int n = min(256, u.count - s0);
-        const float* p = p0 + s0 * step;
-        const float m = tid < n ? p[tid * step] : -INFINITY;
-        const float l = tid < n ? p[tid * step + 1] : 0.0f;
+    for (int s0 = 0; s0 < total; s0 += 256) {
+        const int n = min(256, total - s0);
+        const float* const p = partial(s0 + min(tid, n - 1));
+        const float m = tid < n ? p[0] : -INFINITY;
+        const float l = tid < n ? p[1] : 0.0f;
         const float mw = wave_max(m);
         if (lane == 0) wmax[wave] = mw;
         __syncthreads();
@@ -45,7 +58,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t
         acc *= old;
         if (part < P) {
 #pragma unroll 8
-            for (int s = part; s < n; s += P) acc += fac[s] * p[s * step + 2 + e];
+            for (int s = part; s < n; s += P) acc += fac[s] * partial(s0 + s)[2 + e];
         }
         M = mn;
         __syncthreads();
@@ -66,11 +79,36 @@ struct PagedPlan {
     int G, groups;     // query heads of a workgroup, workgroups per sequence and unit
     int unit_tiles, unit_target;
     int units;         // at most
-    size_t bytes;      // of partials
+    // the shared prefix's kernel (splits 0: the prefix is attended as own keys)
+    int splits, tiles_per, nc, row_waves, row_groups;
+    size_t own_bytes, bytes;   // of the units' partials, and with the prefix's
 };
 
-PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len, int d) {
+// The shared prefix: row blocks of 16 nc query rows, as many to a workgroup as
+// leave the fewest idle (the more the better: they read the same tiles), and
+// one workgroup per CU.
+void plan_prefix(PagedPlan& p, int batch, int n_heads, int n_kv_heads, int shared_len, int d) {
+    const int64_t rows = (int64_t)batch * (n_heads / n_kv_heads);
+    if (shared_len == 0 || batch < 2 || !bc::prefix_dim(d)) return;
+    p.nc = d <= 128 && rows > 16 ? 2 : 1;
+    const int64_t blocks = (rows + 16 * p.nc - 1) / (16 * p.nc);
+    p.row_waves = 1;
+    for (int w = 2; w <= 4; w *= 2)
+        if ((blocks + w - 1) / w * w <= (blocks + p.row_waves - 1) / p.row_waves * p.row_waves) p.row_waves = w;
+    p.row_groups = (int)((blocks + p.row_waves - 1) / p.row_waves);
+    const int tiles = shared_len / 64, wk = 8 / p.row_waves;
+    int64_t splits = bc::device_cu_count() / ((int64_t)n_kv_heads * p.row_groups);
+    if (splits > (tiles + wk - 1) / wk) splits = (tiles + wk - 1) / wk;
+    if (splits < 1) splits = 1;
+    p.tiles_per = (int)((tiles + splits - 1) / splits);
+    if (p.tiles_per > 64 * wk) p.tiles_per = 64 * wk;   // (a wave's tiles sit in one register)
+    p.splits = (tiles + p.tiles_per - 1) / p.tiles_per;
+}
+
+PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len, int shared_len, int d) {
     PagedPlan p{};
+    plan_prefix(p, batch, n_heads, n_kv_heads, shared_len, d);
+    if (p.splits > 0) max_seq_len -= shared_len;   // (units hold the keys after it)
     p.G = bc::attention_group(n_heads / n_kv_heads, d, mode);
     p.groups = n_kv_heads * (n_heads / n_kv_heads / p.G);
     const int64_t tiles = ((int64_t)max_seq_len + 63) / 64;
@@ -80,7 +118,7 @@ PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len
     p.unit_target = (int)((2LL * fit * cu + p.groups - 1) / p.groups);
     // (at least two tiles a wave, one where that leaves CUs idle)
     p.unit_tiles = (int64_t)batch * p.groups * ((tiles + 7) / 8) < cu ? 4 : 8;
-    if (tiles <= p.unit_tiles) {
+    if (tiles <= p.unit_tiles && p.splits == 0) {
         p.unit_tiles = 0;
         p.units = batch;
         return p;
@@ -90,7 +128,8 @@ PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len
     int64_t units = (capped > p.unit_target ? capped : p.unit_target) + batch;
     if (units > most) units = most;
     p.units = (int)units;
-    p.bytes = (size_t)units * n_heads * (d + 2) * sizeof(float);
+    p.own_bytes = (size_t)units * n_heads * (d + 2) * sizeof(float);
+    p.bytes = p.own_bytes + (size_t)p.splits * batch * n_heads * (d + 2) * sizeof(float);
     return p;
 }
 
@@ -104,6 +143,7 @@ int validate(int batch, int n_heads, int n_kv_heads, int max_seq_len, int shared
                "n_heads (%d) must be a multiple of n_kv_heads (%d)", n_heads, n_kv_heads);
     BC_REQUIRE(shared_len <= max_seq_len, BC_ERR_INVALID_ARGUMENT, "shared_len (%d) above max_seq_len (%d)",
                shared_len, max_seq_len);
+    BC_REQUIRE(shared_len % 64 == 0, BC_ERR_INVALID_ARGUMENT, "shared_len (%d) must be whole pages", shared_len);
     BC_REQUIRE(batch <= 65535, BC_ERR_UNSUPPORTED, "batch above 65535");
     BC_REQUIRE(n_heads <= 65535, BC_ERR_UNSUPPORTED, "n_heads above 65535");
     BC_REQUIRE((int64_t)batch * (max_seq_len / 64 + 1) <= INT32_MAX, BC_ERR_UNSUPPORTED,
@@ -121,7 +161,7 @@ extern "C" int bc_paged_attention_workspace_size(int batch, int n_heads, int n_k
     *bytes = 0;
     if ((int64_t)batch * n_heads == 0) return BC_OK;
     for (int mode : {MODE_BINARY, MODE_COMP}) {
-        const size_t n = plan(mode, batch, n_heads, n_kv_heads, max_seq_len, head_dim).bytes;
+        const size_t n = plan(mode, batch, n_heads, n_kv_heads, max_seq_len, shared_len, head_dim).bytes;
         if (n > *bytes) *bytes = n;
     }
     return BC_OK;
@@ -150,10 +190,10 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     BC_REQUIRE(q && out && seq_lens && (table_width == 0 || block_tables) && (n_pages == 0 || (k_bin && v_bin)),
                BC_ERR_INVALID_ARGUMENT, "null pointer");
     const int mode = k_res ? MODE_COMP : MODE_BINARY;
-    const PagedPlan p = plan(mode, batch, n_heads, n_kv_heads, max_seq_len, head_dim);
+    const PagedPlan p = plan(mode, batch, n_heads, n_kv_heads, max_seq_len, shared_len, head_dim);
     BC_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes), BC_ERR_WORKSPACE,
                "workspace of %zu bytes required, got %zu", p.bytes, workspace_bytes);
-    BC_REQUIRE(p.groups <= 65535, BC_ERR_UNSUPPORTED, "more than 65535 head groups");
+    BC_REQUIRE(p.groups <= 65535 && (int64_t)n_kv_heads * p.row_groups <= 65535, BC_ERR_UNSUPPORTED, "more than 65535 head groups");
     const int64_t cap = (int64_t)n_pages * n_kv_heads * page_size;
     hipStream_t st = (hipStream_t)stream;
     AttnArgs a{};
@@ -175,15 +215,31 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     a.unit_tiles = p.unit_tiles;
     a.unit_target = p.unit_target;
     a.bf16 = dtype == BC_BF16;
+    float* const prefix_ws = (float*)((uint8_t*)workspace + p.own_bytes);
+    if (p.splits > 0) {
+        // (no page of a pool without pages is read: its splits' rows are not used)
+        a.key0 = shared_len;
+        const PrefixArgs x{prefix_ws, n_pages > 0 ? shared_len / 64 : 0, p.tiles_per, p.row_waves};
+        const dim3 grid(p.splits, n_kv_heads * p.row_groups);
+        int st_prefix = BC_ERR_UNSUPPORTED;
+        switch (head_dim) {
+#define BC_CASE(DD) case DD: st_prefix = bc::prefix_launch<DD>(k_res != nullptr, p.nc, a, x, grid, st); break;
+            BC_CASE(64) BC_CASE(128) BC_CASE(192) BC_CASE(256)
+#undef BC_CASE
+            default: break;
+        }
+        if (st_prefix != BC_OK) return st_prefix;
+    }
     if (p.unit_tiles == 0) a.out = (uint16_t*)out;
-    BC_REQUIRE(bc::launch_paged_split(mode, head_dim, p.G, a, dim3(p.units, p.groups), st), BC_ERR_UNSUPPORTED,
-               "head_dim %d", head_dim);
+    if (p.units > 0)
+        BC_REQUIRE(bc::launch_paged_split(mode, head_dim, p.G, a, dim3(p.units, p.groups), st), BC_ERR_UNSUPPORTED,
+                   "head_dim %d", head_dim);
     const int launched = bc::check_launch("paged attention");
     if (launched != BC_OK || p.unit_tiles == 0) return launched;
     const dim3 grid(n_heads, batch);
     switch (head_dim) {
 #define BC_CASE(DD) \
-    case DD: hipLaunchKernelGGL((paged_combine_kernel<DD>), grid, dim3(256), 0, st, a, (uint16_t*)out); break;
+    case DD: hipLaunchKernelGGL((paged_combine_kernel<DD>), grid, dim3(256), 0, st, a, (uint16_t*)out, prefix_ws, p.splits); break;
         BC_CASE(32) BC_CASE(64) BC_CASE(96) BC_CASE(128) BC_CASE(160) BC_CASE(192) BC_CASE(224) BC_CASE(256)
 #undef BC_CASE
         default: return bc::set_error(BC_ERR_UNSUPPORTED, "head_dim %d", head_dim);

@@ -72,6 +72,18 @@ def test_paged_attention_argument_errors(lib, no_gpu):  # noqa: F811
     assert w(4, 8, 2, 1000, 0, 80, ctypes.byref(n)) == BC_ERR_UNSUPPORTED
     assert w(-1, 8, 2, 1000, 0, 128, ctypes.byref(n)) == BC_ERR_INVALID_ARGUMENT
     assert w(4, 8, 2, 1000, 1024, 128, ctypes.byref(n)) == BC_ERR_INVALID_ARGUMENT
+    assert w(4, 8, 2, 1000, 32, 128, ctypes.byref(n)) == BC_ERR_INVALID_ARGUMENT
+    # every shape has a plan, and a shared prefix's partials are in it
+    for B in (1, 2, 3, 17, 64, 500, 65535):
+        for H, Hkv in ((1, 1), (8, 2), (24, 8), (64, 1), (32, 32)):
+            for longest in (0, 1, 64, 65, 1000, 131072):
+                for shared in (0, 64, 640, 65536):
+                    for d in (32, 64, 96, 128, 160, 192, 224, 256):
+                        if shared <= longest and B * (longest // 64 + 1) < 2 ** 31:
+                            assert w(B, H, Hkv, longest, shared, d, ctypes.byref(n)) == BC_OK
+    assert w(64, 32, 8, 34816, 0, 128, ctypes.byref(n)) == BC_OK
+    alone = n.value
+    assert w(64, 32, 8, 34816, 32768, 128, ctypes.byref(n)) == BC_OK and n.value > 64 * 32 * 130 * 4 and alone > 0
 
     def call(q=X, kb=X, kr=X, vr=X, tables=X, width=20, lens=X, out=X, B=4, H=8, Hkv=2, pages=50, page=64, longest=1000,
              shared=0, d=128, dtype=0, ws=P(0x10000), size=1 << 40):
