@@ -181,6 +181,11 @@ int paged_wgs_per_cu(int mode, int D, int G);
 // device (0 when no MFMA kernel handles it).
 int mfma_wgs_per_cu(int mode, int D, int G);
 
+// An fp16 value, or a bf16 one where bf is all ones (0 else)
+__device__ __forceinline__ float half_f(uint16_t h, uint32_t bf) {
+    return __builtin_bit_cast(float, ((uint32_t)h << 16 & bf) | (__builtin_bit_cast(uint32_t, h2f(h)) & ~bf));
+}
+
 // Query heads that one workgroup attends for, of the `group` that share a kv head.
 int attention_group(int group, int D, int mode);
 

@@ -253,7 +253,7 @@ __device__ __forceinline__ void lds_barrier() {
 // 16.5 inlined, compensated 49.6 and 43.4).
 template <int D, int G, bool KMF, bool RES, int NT, int NQ>
 __device__ __forceinline__ void prep_digits(const uint16_t (&qpre)[NQ], QDigits<D, G, KMF>& qd, float* qf,
-                                            bool bf16 = false) {
+                                            uint32_t bf = 0u) {
     const int tid = threadIdx.x, lane = tid & 63;
     uint32_t* signs = &qd.signs[0][0];   // [G * D / 32] words, bit b of word i = element 32i + b
     __shared__ float gmax[G * D / 32];   // max |q| of each 32-element group (one head's)
@@ -266,7 +266,7 @@ __device__ __forceinline__ void prep_digits(const uint16_t (&qpre)[NQ], QDigits<
     for (int j = 0; j < NQ; j++) {
         const int i = tid + NT * j;
         if (i - lane >= G * D) break;   // (uniform)
-        const float x = bf16 ? __builtin_bit_cast(float, (uint32_t)qpre[j] << 16) : h2f(qpre[j]);
+        const float x = bc::half_f(qpre[j], bf);
         const uint64_t bits = __ballot(x >= 0.0f);
         const float wm = half_max(fabsf(x));
         if (i < G * D) {
@@ -809,7 +809,7 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
         app_raw = bc::load_row_slice((lane / AL == 1 ? a.app_v : a.app_k) + (int64_t)bkv * D, lane % AL);
         __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (PG) prep_digits<D, G, KMF, RES, NT>(qpre, qd, qf, a.bf16 != 0);
+    if constexpr (PG) prep_digits<D, G, KMF, RES, NT>(qpre, qd, qf, a.bf16 ? 0xFFFFFFFFu : 0u);
     else prep_digits<D, G, KMF, RES, NT>(qpre, qd, qf);
 
     // In-place append: the wave that takes the slot's tile encodes the token's

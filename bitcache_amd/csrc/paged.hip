@@ -7,10 +7,10 @@
 #include "prefix_attn.h"
 
 namespace bc {
-extern template int prefix_launch<64>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
-extern template int prefix_launch<128>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
-extern template int prefix_launch<192>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
-extern template int prefix_launch<256>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+extern template void prefix_launch<64>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+extern template void prefix_launch<128>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+extern template void prefix_launch<192>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+extern template void prefix_launch<256>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
 }  // namespace bc
 
 namespace {
@@ -80,28 +80,21 @@ struct PagedPlan {
     int unit_tiles, unit_target;
     int units;         // at most
     // the shared prefix's kernel (splits 0: the prefix is attended as own keys)
-    int splits, tiles_per, nc, row_waves, row_groups;
+    int splits, tiles_per, nc, row_groups;
     size_t own_bytes, bytes;   // of the units' partials, and with the prefix's
 };
 
-// The shared prefix: row blocks of 16 nc query rows, as many to a workgroup as
-// leave the fewest idle (the more the better: they read the same tiles), and
-// one workgroup per CU.
+// The shared prefix: groups of 16 nc query rows, and two workgroups per CU.
 void plan_prefix(PagedPlan& p, int batch, int n_heads, int n_kv_heads, int shared_len, int d) {
     const int64_t rows = (int64_t)batch * (n_heads / n_kv_heads);
     if (shared_len == 0 || batch < 2 || !bc::prefix_dim(d)) return;
-    p.nc = d <= 128 && rows > 16 ? 2 : 1;
-    const int64_t blocks = (rows + 16 * p.nc - 1) / (16 * p.nc);
-    p.row_waves = 1;
-    for (int w = 2; w <= 4; w *= 2)
-        if ((blocks + w - 1) / w * w <= (blocks + p.row_waves - 1) / p.row_waves * p.row_waves) p.row_waves = w;
-    p.row_groups = (int)((blocks + p.row_waves - 1) / p.row_waves);
-    const int tiles = shared_len / 64, wk = 8 / p.row_waves;
-    int64_t splits = bc::device_cu_count() / ((int64_t)n_kv_heads * p.row_groups);
-    if (splits > (tiles + wk - 1) / wk) splits = (tiles + wk - 1) / wk;
+    p.nc = rows <= 16 ? 1 : rows <= 32 ? 2 : bc::prefix_columns(d);
+    p.row_groups = (int)((rows + 16 * p.nc - 1) / (16 * p.nc));
+    const int tiles = shared_len / 64;
+    int64_t splits = 2LL * bc::device_cu_count() / ((int64_t)n_kv_heads * p.row_groups);
+    if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
     if (splits < 1) splits = 1;
     p.tiles_per = (int)((tiles + splits - 1) / splits);
-    if (p.tiles_per > 64 * wk) p.tiles_per = 64 * wk;   // (a wave's tiles sit in one register)
     p.splits = (tiles + p.tiles_per - 1) / p.tiles_per;
 }
 
@@ -216,19 +209,20 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     a.unit_target = p.unit_target;
     a.bf16 = dtype == BC_BF16;
     float* const prefix_ws = (float*)((uint8_t*)workspace + p.own_bytes);
-    if (p.splits > 0) {
-        // (no page of a pool without pages is read: its splits' rows are not used)
-        a.key0 = shared_len;
-        const PrefixArgs x{prefix_ws, n_pages > 0 ? shared_len / 64 : 0, p.tiles_per, p.row_waves};
+    // (a pool without pages holds no length but zero: nothing to attend)
+    const int splits = n_pages > 0 ? p.splits : 0;
+    if (p.splits > 0) a.key0 = shared_len;
+    if (splits > 0) {
+        const PrefixArgs x{prefix_ws, shared_len / 64, p.tiles_per};
         const dim3 grid(p.splits, n_kv_heads * p.row_groups);
-        int st_prefix = BC_ERR_UNSUPPORTED;
         switch (head_dim) {
-#define BC_CASE(DD) case DD: st_prefix = bc::prefix_launch<DD>(k_res != nullptr, p.nc, a, x, grid, st); break;
+#define BC_CASE(DD) case DD: bc::prefix_launch<DD>(k_res != nullptr, p.nc, a, x, grid, st); break;
             BC_CASE(64) BC_CASE(128) BC_CASE(192) BC_CASE(256)
 #undef BC_CASE
-            default: break;
+            default: return bc::set_error(BC_ERR_UNSUPPORTED, "head_dim %d", head_dim);
         }
-        if (st_prefix != BC_OK) return st_prefix;
+        const int prefix_rc = bc::check_launch("prefix attention");
+        if (prefix_rc != BC_OK) return prefix_rc;
     }
     if (p.unit_tiles == 0) a.out = (uint16_t*)out;
     if (p.units > 0)
@@ -239,7 +233,7 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     const dim3 grid(n_heads, batch);
     switch (head_dim) {
 #define BC_CASE(DD) \
-    case DD: hipLaunchKernelGGL((paged_combine_kernel<DD>), grid, dim3(256), 0, st, a, (uint16_t*)out, prefix_ws, p.splits); break;
+    case DD: hipLaunchKernelGGL((paged_combine_kernel<DD>), grid, dim3(256), 0, st, a, (uint16_t*)out, prefix_ws, splits); break;
         BC_CASE(32) BC_CASE(64) BC_CASE(96) BC_CASE(128) BC_CASE(160) BC_CASE(192) BC_CASE(224) BC_CASE(256)
 #undef BC_CASE
         default: return bc::set_error(BC_ERR_UNSUPPORTED, "head_dim %d", head_dim);

@@ -9,13 +9,15 @@ struct PrefixArgs {
     float* ws;        // [splits][B * Hq][D + 2] partials: m (log2 domain), l, acc[D]
     int tiles;        // 64-key tiles of the prefix (tables' first row)
     int tiles_per;    // tiles of a split
-    int row_waves;    // row blocks of a workgroup: 1, 2, 4 or 8
 };
 
-// Head dims with instances, and the rows of a row block there (in sixteens)
+// Head dims with instances, and a workgroup's rows there at most (in sixteens):
+// what holds the rows' operands and sums in registers at two waves per SIMD
 constexpr bool prefix_dim(int d) { return d % 64 == 0; }
-// grid.x splits, grid.y kv heads times row-block groups
+constexpr int prefix_columns(int d) { return d <= 128 ? 4 : 2; }
+// nc 1, 2 or 4 (at most prefix_columns): 16 nc rows per workgroup; grid.x splits,
+// grid.y kv heads times groups of rows
 template <int D>
-int prefix_launch(bool res, int nc, const AttnArgs& a, const PrefixArgs& x, dim3 grid, hipStream_t st);
+void prefix_launch(bool res, int nc, const AttnArgs& a, const PrefixArgs& x, dim3 grid, hipStream_t st);
 
 }  // namespace bc

@@ -2,5 +2,5 @@
 #include "prefix_attn_kernel.h"
 
 namespace bc {
-template int prefix_launch<256>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
+template void prefix_launch<256>(bool, int, const AttnArgs&, const PrefixArgs&, dim3, hipStream_t);
 }  // namespace bc
