@@ -54,19 +54,25 @@ struct AttnArgs {
     const int32_t* tables;
     int width, n_pages, page_tiles, key0, max_len;
     int unit_tiles;   // see PagedUnit; 0: one unit per sequence
-    int unit_target;
+    int unit_slots, unit_most;
     int bf16;         // queries and outputs are bf16
 };
 
-// Work units of a paged call: a sequence's tiles after key0 are cut into units of
-// equal size, as many as bring a unit to at most `chunk` tiles, where chunk is
-// the batch's tiles over unit_target units, at least unit_tiles (and at most
-// kUnitTiles: a wave holds its tiles' places in one register).  A batch of
-// any lengths then is at most max(unit_target, batch * tiles / kUnitTiles) +
-// batch units of nearly the same size, and the launch is planned without
-// knowing the lengths.  unit_tiles = 0: unit b is sequence b.  Each wave finds its unit by
-// itself from the lengths (one load per 64 sequences and two wave scans).
-constexpr int kUnitTiles = 256;
+// Work units of a paged call.  A sequence's tiles after key0 are cut into units of
+// equal size, as many as bring a unit to at most `chunk` tiles; the device
+// chooses chunk from the lengths, so that the launch is planned without knowing
+// them and a captured call follows them.  unit_slots units (times the head
+// groups) run at once.  Eight candidates aim at half to two rounds of them, and
+// the one with the least rounds * (mean unit + kUnitFixed) is taken (the fixed
+// work of a unit, its query preparation, merge and first loads, is that of four
+// tiles), as far as its units fit the launched ones (unit_most); chunk is at
+// least unit_tiles and at most kUnitTiles (a wave holds its tiles' places in one
+// register), which always fits.  unit_tiles = 0: unit b is sequence b.  Each wave
+// finds its unit by itself.  (64 sequences of 128 to 32768 keys, 32/8 heads: 119
+// us; the candidates taken alone 112 to 124, those that do not fit 180; one equal
+// range of tiles per slot, across sequences, 159: two segments in most ranges,
+// each with the fixed work and none beside another's loop.)
+constexpr int kUnitTiles = 256, kUnitFixed = 4, kUnitRounds = 2;
 struct PagedUnit {
     int b, len;        // (b < 0: no such unit)
     int first, tiles;  // the unit's tiles, counted from key0
@@ -90,30 +96,63 @@ __device__ __forceinline__ int wave_scan_add(int v) {
 #undef BC_SCAN_STEP
     return v;
 }
-// Tiles of a unit at most
-__device__ __forceinline__ int paged_chunk(const AttnArgs& a, int lane) {
-    int n = 0;
-    for (int i = lane; i < a.B; i += 64) n += paged_tiles(a, a.lens[i]);
+// Units at most, of a batch of `tiles` tiles at most
+__host__ __device__ inline int64_t paged_unit_most(int slots, int batch, int64_t tiles) {
+    const int64_t full = (int64_t)kUnitRounds * slots, capped = (tiles + kUnitTiles - 1) / kUnitTiles + batch;
+    return capped > full ? capped : full;
+}
+// Tiles of a unit at most.  own: the tiles of sequence `lane` (0 past the batch).
+__device__ __forceinline__ int paged_chunk(const AttnArgs& a, int lane, int& own) {
+    own = lane < a.B ? paged_tiles(a, a.lens[lane]) : 0;
+    int n = own;
+    for (int i = lane + 64; i < a.B; i += 64) n += paged_tiles(a, a.lens[i]);
     const int total = __builtin_amdgcn_readlane(wave_scan_add(n), 63);
-    return min(max((total + a.unit_target - 1) / a.unit_target, a.unit_tiles), kUnitTiles);
+    // lane = (candidate, eighth of the sequences); candidates in 16ths of a round
+    const int cand = lane & 7;
+    const int sixteenths = (int)(0x20181410'0F0E0C08ull >> (8 * cand)) & 0xFF;
+    const float even = ceilf(16.0f * (float)total / ((float)a.unit_slots * (float)sixteenths));
+    const int chunk = max((int)fminf(even, (float)kUnitTiles), a.unit_tiles);
+    const float inv = 1.0f / (float)chunk;
+    int units = 0;
+    for (int i0 = 0; i0 < a.B; i0 += 64) {
+        const int t = i0 == 0 ? own : i0 + lane < a.B ? paged_tiles(a, a.lens[i0 + lane]) : 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            // (the quotient within one, then exact: the launch holds the units)
+            const int x = __builtin_amdgcn_ds_bpermute(4 * (8 * k + (lane >> 3)), t), n = (int)((float)x * inv);
+            const int rest = x - n * chunk;
+            units += n + (rest > 0) + (rest > chunk);
+        }
+    }
+    // (the eighths: lanes 8, 16 and 32 apart)
+    units += __builtin_amdgcn_ds_swizzle(units, 0x201F);
+    units += __builtin_amdgcn_ds_swizzle(units, 0x401F);
+    units += __builtin_amdgcn_ds_bpermute(4 * (lane ^ 32), units);
+    const float rounds = ceilf((float)units / (float)a.unit_slots);
+    const float tiles = rounds * ((float)total / (float)max(units, 1) + (float)kUnitFixed);
+    uint32_t cost[1] = {~((uint32_t)fminf(16.0f * tiles, 268435455.0f) << 3 | (uint32_t)cand)};
+    if (units > a.unit_most) cost[0] = 0;
+    wave_umax(cost);
+    return cost[0] == 0 ? kUnitTiles : __builtin_amdgcn_readlane(chunk, (int)(~cost[0] & 7));
 }
 __device__ __forceinline__ PagedUnit paged_unit(const AttnArgs& a, int unit, int lane) {
     if (a.unit_tiles == 0) {
         const int len = __builtin_amdgcn_readfirstlane(a.lens[unit]);
         return PagedUnit{unit, len, 0, paged_tiles(a, len)};
     }
-    const int chunk = paged_chunk(a, lane);
+    int own;
+    const int chunk = paged_chunk(a, lane, own);
     int base = 0;
     for (int i0 = 0; i0 < a.B; i0 += 64) {
-        const int len = i0 + lane < a.B ? a.lens[i0 + lane] : 0;
-        const int tiles = paged_tiles(a, len), n = (tiles + chunk - 1) / chunk;
+        const int tiles = i0 == 0 ? own : i0 + lane < a.B ? paged_tiles(a, a.lens[i0 + lane]) : 0;
+        const int n = (tiles + chunk - 1) / chunk;
         const int incl = wave_scan_add(n), last = __builtin_amdgcn_readlane(incl, 63);
         if (unit - base < last) {
             const int at = __builtin_ctzll(__ballot(incl > unit - base));
             const int mine = __builtin_amdgcn_readlane(tiles, at), count = __builtin_amdgcn_readlane(n, at);
             const int split = unit - base - (__builtin_amdgcn_readlane(incl, at) - count);
             const int per = (mine + count - 1) / count;
-            return PagedUnit{i0 + at, __builtin_amdgcn_readlane(len, at), split * per, min(per, mine - split * per)};
+            return PagedUnit{i0 + at, __builtin_amdgcn_readfirstlane(a.lens[i0 + at]), split * per, max(0, min(per, mine - split * per))};
         }
         base += last;
     }
@@ -124,10 +163,12 @@ struct PagedUnits {
     int first, count;
 };
 __device__ __forceinline__ PagedUnits paged_units(const AttnArgs& a, int b, int lane) {
-    const int chunk = paged_chunk(a, lane);
+    int own;
+    const int chunk = paged_chunk(a, lane, own);
     int base = 0;
     for (int i0 = 0;; i0 += 64) {
-        const int tiles = i0 + lane < a.B ? paged_tiles(a, a.lens[i0 + lane]) : 0, n = (tiles + chunk - 1) / chunk;
+        const int tiles = i0 == 0 ? own : i0 + lane < a.B ? paged_tiles(a, a.lens[i0 + lane]) : 0;
+        const int n = (tiles + chunk - 1) / chunk;
         const int incl = wave_scan_add(n);
         if (b < i0 + 64) {
             const int count = __builtin_amdgcn_readlane(n, b - i0);
@@ -167,8 +208,9 @@ bool mfma_split_ok(int D, int64_t chunk, int64_t head_groups);
 // Head dims whose kernels append a token in place (the one-slice row encoder
 // of encode_row.h takes power-of-two lane groups).
 __host__ __device__ constexpr bool append_dim(int D) { return D == 64 || D == 128 || D == 256; }
-// The paged instances (binary and compensated modes): grid.x units, grid.y kv
-// heads times query-head groups of a kv head; the partial of unit u and query
+// The paged instances (binary and compensated modes): grid.x kv heads times
+// query-head groups of a kv head, grid.y units (those past the batch's last one,
+// which leave at once, come last); the partial of unit u and query
 // head h goes to ws[(u * Hq + h) * (D + 2)], or the outputs to a.out (one unit per
 // sequence).
 template <int D>

@@ -473,8 +473,8 @@ __host__ __device__ constexpr bool k_on_mfma(int G, int mode) {
 // APP: the workgroup whose key range holds the slot a.app_slot appends the
 // token a.app_k / a.app_v there.
 // PG: a paged cache (kv_rows pages times kv heads, kv_stride the page size): the
-// workgroup takes work unit blockIdx.x (PagedUnit) of kv head and group
-// blockIdx.y; a tile lies in one page, so each tile's loads go through buffer
+// workgroup takes work unit blockIdx.y (PagedUnit) of kv head and group
+// blockIdx.x; a tile lies in one page, so each tile's loads go through buffer
 // resources of its own, over its keys alone.
 //
 // The scalar arguments (14 dwords) come in registers with the wave (kernarg
@@ -584,9 +584,9 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
     __shared__ float wfac[G == 8 ? NW : 1][G], wtot[G == 8 ? 2 : 1][G];
     __shared__ int wbad[PG ? NW : 1];   // (paged) the wave met a page outside the pool
 
-    const int split = blockIdx.x;
+    const int split = PG ? blockIdx.y : blockIdx.x;
     // per-head modes: this launch's query-head groups come from its list
-    int grow = blockIdx.y;
+    int grow = PG ? blockIdx.x : blockIdx.y;
     if constexpr (MODE == MODE_BINARY || MODE == MODE_MIXED) {
         if (plan & kPlanList) {
             if (grow >= *a.group_count) return;

@@ -19,79 +19,112 @@ using bc::PrefixArgs;
 using bc::MODE_BINARY;
 using bc::MODE_COMP;
 
-// The merge of a sequence's units, and of the shared prefix's splits (prefix:
-// `splits` partials per row): one workgroup per (sequence, query head), the
-// partials spread over its 256 / D groups of threads (one of at least D).
-template <int D>
+// The merge of a sequence's units, and of the shared prefix's `splits` partials per
+// row: PARTS waves per (sequence, query head), each over every PARTS-th partial
+// (lane = partial for the factors, lanes = dims for the sums), joined in LDS.
+// Bound: the latency of its three loads in turn (lengths, maxima, sums).
+template <int D, int PARTS>
 __global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t* out, const float* prefix, int splits) {
-    constexpr int P = 256 / D;
-    __shared__ float fac[256];
-    __shared__ float red[P * D];
-    __shared__ float wmax[4], wsum[4];
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int N = (D + 63) / 64;     // dims of a lane
+    constexpr int ROWS = 4 / PARTS;      // rows of a workgroup
+    __shared__ float join[PARTS > 1 ? 4 : 1][D + 2];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int part = wave % PARTS;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + wave / PARTS;
+    const bool live = row < (int64_t)a.B * a.Hq;
+    const int b = live ? (int)(row / a.Hq) : 0, h = live ? (int)(row - (int64_t)b * a.Hq) : 0;
     const bc::PagedUnits u = bc::paged_units(a, b, lane);
     const int64_t own_step = (int64_t)a.Hq * (D + 2), prefix_step = own_step * a.B;
-    const float* own = a.ws + (int64_t)u.first * own_step + (int64_t)h * (D + 2);
-    const float* shared = prefix + ((int64_t)b * a.Hq + h) * (D + 2);
-    const int total = splits + u.count;
-    auto partial = [&](int s) { return s < splits ? shared + s * prefix_step : own + (s - splits) * own_step; };
-    const int part = tid / D, e = tid % D;
-    // online over blocks of 256 partials
-    float M = -INFINITY, L = 0.0f, acc = 0.0f;
-    for (int s0 = 0; s0 < total; s0 += 256) {
-        const int n = min(256, total - s0);
-        const float* const p = partial(s0 + min(tid, n - 1));
-        const float m = tid < n ? p[0] : -INFINITY;
-        const float l = tid < n ? p[1] : 0.0f;
-        const float mw = wave_max(m);
-        if (lane == 0) wmax[wave] = mw;
-        __syncthreads();
-        const float mn = fmaxf(fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3])), M);
-        const float f = m == -INFINITY ? 0.0f : exp2f(m - mn);
-        fac[tid] = f;
-        // (a NaN sum marks a bad page: it stays one at any factor)
-        const float lw = wave_sum(l == l ? f * l : l);
-        if (lane == 0) wsum[wave] = lw;
-        __syncthreads();
-        const float old = M == -INFINITY ? 0.0f : exp2f(M - mn);
-        L = L * old + ((wsum[0] + wsum[1]) + (wsum[2] + wsum[3]));
-        acc *= old;
-        if (part < P) {
-#pragma unroll 8
-            for (int s = part; s < n; s += P) acc += fac[s] * partial(s0 + s)[2 + e];
-        }
-        M = mn;
-        __syncthreads();
-    }
-    if (part < P) red[part * D + e] = acc;
-    __syncthreads();
-    if (tid < D) {
-        float o = red[tid];
+    const float* const own = a.ws + (int64_t)u.first * own_step + (int64_t)h * (D + 2);
+    const float* const shared = prefix + ((int64_t)b * a.Hq + h) * (D + 2);
+    const int total = live ? splits + u.count : 0;
+    // (s-th partial of this wave)
+    auto partial = [&](int s) {
+        s = s * PARTS + part;
+        return s < splits ? shared + s * prefix_step : own + (s - splits) * own_step;
+    };
+    const int mine = (total - part + PARTS - 1) / PARTS;
+    float M = -INFINITY, L = 0.0f, acc[N];
 #pragma unroll
-        for (int q = 1; q < P; q++) o += red[q * D + tid];
-        // (NaN where the length is out of bounds)
-        o = bc::paged_bad_len(a, a.lens[b]) ? __builtin_nanf("") : L == 0.0f ? 0.0f : o * (1.0f / L);
-        out[((int64_t)b * a.Hq + h) * D + tid] = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o) : f2h(o);
+    for (int n = 0; n < N; n++) acc[n] = 0.0f;
+    for (int s0 = 0; s0 < mine; s0 += 64) {
+        const int cnt = min(64, mine - s0);
+        const float* const p = partial(s0 + min(lane, cnt - 1));
+        const float m = lane < cnt ? p[0] : -INFINITY, l = lane < cnt ? p[1] : 0.0f;
+        const float mn = fmaxf(wave_max(m), M);
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        const float old = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
+        // (a NaN sum marks a bad page: it stays one at any factor)
+        L = L * old + wave_sum(l == l ? f * l : l);
+        M = mn;
+#pragma unroll
+        for (int n = 0; n < N; n++) acc[n] *= old;
+#pragma unroll 8
+        for (int s = 0; s < cnt; s++) {
+            const float* const q = partial(s0 + s) + 2 + lane;
+            const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
+#pragma unroll
+            for (int n = 0; n < N; n++)
+                if (D % 64 == 0 || n < N - 1 || lane < 32) acc[n] = fmaf(fs, q[64 * n], acc[n]);
+        }
     }
+    if constexpr (PARTS > 1) {
+#pragma unroll
+        for (int n = 0; n < N; n++)
+            if (64 * n + lane < D) join[wave][64 * n + lane] = acc[n];
+        if (lane == 0) {
+            join[wave][D] = M;
+            join[wave][D + 1] = L;
+        }
+        __syncthreads();
+        if (part != 0) return;
+        const int w0 = wave;
+        float m[PARTS], top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PARTS; w++) {
+            m[w] = join[w0 + w][D];
+            top = fmaxf(top, m[w]);
+        }
+        L = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; n++) acc[n] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < PARTS; w++) {
+            const float f = m[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[w] - top), l = join[w0 + w][D + 1];
+            L += l == l ? f * l : l;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+                if (64 * n + lane < D) acc[n] = fmaf(f, join[w0 + w][64 * n + lane], acc[n]);
+        }
+    }
+    if (!live) return;
+    const bool bad = bc::paged_bad_len(a, a.lens[b]);   // (NaN where the length is out of bounds)
+    const float inv = bad ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int n = 0; n < N; n++)
+        if (64 * n + lane < D) {
+            const float o = acc[n] * inv;
+            out[row * D + 64 * n + lane] = a.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)o) : f2h(o);
+        }
 }
 
 struct PagedPlan {
     int G, groups;     // query heads of a workgroup, workgroups per sequence and unit
-    int unit_tiles, unit_target;
+    int unit_tiles, unit_slots;
     int units;         // at most
     // the shared prefix's kernel (splits 0: the prefix is attended as own keys)
     int splits, tiles_per, nc, row_groups;
     size_t own_bytes, bytes;   // of the units' partials, and with the prefix's
 };
 
-// The shared prefix: groups of 16 nc query rows, and two workgroups per CU.
-void plan_prefix(PagedPlan& p, int batch, int n_heads, int n_kv_heads, int shared_len, int d) {
+// The shared prefix: groups of 16 nc query rows, and as many workgroups as the CUs hold.
+void plan_prefix(PagedPlan& p, int mode, int batch, int n_heads, int n_kv_heads, int shared_len, int d) {
     const int64_t rows = (int64_t)batch * (n_heads / n_kv_heads);
     if (shared_len == 0 || batch < 2 || !bc::prefix_dim(d)) return;
     p.nc = rows <= 16 ? 1 : rows <= 32 ? 2 : bc::prefix_columns(d);
     p.row_groups = (int)((rows + 16 * p.nc - 1) / (16 * p.nc));
     const int tiles = shared_len / 64;
-    int64_t splits = 2LL * bc::device_cu_count() / ((int64_t)n_kv_heads * p.row_groups);
+    int64_t splits = (int64_t)bc::prefix_waves(d, p.nc, mode != MODE_BINARY) * bc::device_cu_count() / ((int64_t)n_kv_heads * p.row_groups);
     if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
     if (splits < 1) splits = 1;
     p.tiles_per = (int)((tiles + splits - 1) / splits);
@@ -100,25 +133,25 @@ void plan_prefix(PagedPlan& p, int batch, int n_heads, int n_kv_heads, int share
 
 PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len, int shared_len, int d) {
     PagedPlan p{};
-    plan_prefix(p, batch, n_heads, n_kv_heads, shared_len, d);
+    plan_prefix(p, mode, batch, n_heads, n_kv_heads, shared_len, d);
     if (p.splits > 0) max_seq_len -= shared_len;   // (units hold the keys after it)
     p.G = bc::attention_group(n_heads / n_kv_heads, d, mode);
     p.groups = n_kv_heads * (n_heads / n_kv_heads / p.G);
     const int64_t tiles = ((int64_t)max_seq_len + 63) / 64;
-    const int cu = bc::device_cu_count();
-    int fit = bc::paged_wgs_per_cu(mode, d, p.G);
-    if (fit <= 0) fit = 3;
-    p.unit_target = (int)((2LL * fit * cu + p.groups - 1) / p.groups);
-    // (at least two tiles a wave, one where that leaves CUs idle)
-    p.unit_tiles = (int64_t)batch * p.groups * ((tiles + 7) / 8) < cu ? 4 : 8;
-    if (tiles <= p.unit_tiles && p.splits == 0) {
-        p.unit_tiles = 0;
+    // short sequences: one unit each, and no merge (4 sequences of 100 to 1024 keys:
+    // 12 us, 18.7 us in units)
+    if (tiles <= 16 && p.splits == 0) {
         p.units = batch;
         return p;
     }
+    const int cu = bc::device_cu_count();
+    int fit = bc::paged_wgs_per_cu(mode, d, p.G);
+    if (fit <= 0) fit = 3;
+    p.unit_slots = (int)(((int64_t)fit * cu + p.groups - 1) / p.groups);
+    // (at least two tiles a wave, one where that leaves CUs idle)
+    p.unit_tiles = (int64_t)batch * p.groups * ((tiles + 7) / 8) < cu ? 4 : 8;
     const int64_t most = (int64_t)batch * ((tiles + p.unit_tiles - 1) / p.unit_tiles);
-    const int64_t capped = ((int64_t)batch * tiles + bc::kUnitTiles - 1) / bc::kUnitTiles;
-    int64_t units = (capped > p.unit_target ? capped : p.unit_target) + batch;
+    int64_t units = bc::paged_unit_most(p.unit_slots, batch, batch * tiles);
     if (units > most) units = most;
     p.units = (int)units;
     p.own_bytes = (size_t)units * n_heads * (d + 2) * sizeof(float);
@@ -184,9 +217,10 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
                BC_ERR_INVALID_ARGUMENT, "null pointer");
     const int mode = k_res ? MODE_COMP : MODE_BINARY;
     const PagedPlan p = plan(mode, batch, n_heads, n_kv_heads, max_seq_len, shared_len, head_dim);
+    BC_REQUIRE(p.units <= 65535, BC_ERR_UNSUPPORTED, "more than 65535 work units");
     BC_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes), BC_ERR_WORKSPACE,
                "workspace of %zu bytes required, got %zu", p.bytes, workspace_bytes);
-    BC_REQUIRE(p.groups <= 65535 && (int64_t)n_kv_heads * p.row_groups <= 65535, BC_ERR_UNSUPPORTED, "more than 65535 head groups");
+    BC_REQUIRE((int64_t)n_kv_heads * p.row_groups <= 65535, BC_ERR_UNSUPPORTED, "more than 65535 head and row groups");
     const int64_t cap = (int64_t)n_pages * n_kv_heads * page_size;
     hipStream_t st = (hipStream_t)stream;
     AttnArgs a{};
@@ -206,7 +240,8 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     a.page_tiles = page_size / 64;
     a.max_len = n_pages > 0 ? max_seq_len : 0;   // (without pages no length but zero is right)
     a.unit_tiles = p.unit_tiles;
-    a.unit_target = p.unit_target;
+    a.unit_slots = p.unit_slots;
+    a.unit_most = p.units;
     a.bf16 = dtype == BC_BF16;
     float* const prefix_ws = (float*)((uint8_t*)workspace + p.own_bytes);
     // (a pool without pages holds no length but zero: nothing to attend)
@@ -226,14 +261,23 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     }
     if (p.unit_tiles == 0) a.out = (uint16_t*)out;
     if (p.units > 0)
-        BC_REQUIRE(bc::launch_paged_split(mode, head_dim, p.G, a, dim3(p.units, p.groups), st), BC_ERR_UNSUPPORTED,
+        BC_REQUIRE(bc::launch_paged_split(mode, head_dim, p.G, a, dim3(p.groups, p.units), st), BC_ERR_UNSUPPORTED,
                    "head_dim %d", head_dim);
     const int launched = bc::check_launch("paged attention");
     if (launched != BC_OK || p.unit_tiles == 0) return launched;
-    const dim3 grid(n_heads, batch);
+    // (four waves a row while the device's wave slots hold them: 2.4 and 2.1 us less
+    // over 512 and 2048 rows of 30 partials)
+    const int64_t rows = (int64_t)batch * n_heads;
+    const bool four = rows < 16LL * bc::device_cu_count();
+    const dim3 grid((unsigned)(four ? rows : (rows + 3) / 4));
     switch (head_dim) {
-#define BC_CASE(DD) \
-    case DD: hipLaunchKernelGGL((paged_combine_kernel<DD>), grid, dim3(256), 0, st, a, (uint16_t*)out, prefix_ws, splits); break;
+#define BC_CASE(DD)                                                                                                   \
+    case DD:                                                                                                          \
+        if (four)                                                                                                     \
+            hipLaunchKernelGGL((paged_combine_kernel<DD, 4>), grid, dim3(256), 0, st, a, (uint16_t*)out, prefix_ws, splits); \
+        else                                                                                                          \
+            hipLaunchKernelGGL((paged_combine_kernel<DD, 1>), grid, dim3(256), 0, st, a, (uint16_t*)out, prefix_ws, splits); \
+        break;
         BC_CASE(32) BC_CASE(64) BC_CASE(96) BC_CASE(128) BC_CASE(160) BC_CASE(192) BC_CASE(224) BC_CASE(256)
 #undef BC_CASE
         default: return bc::set_error(BC_ERR_UNSUPPORTED, "head_dim %d", head_dim);

@@ -15,6 +15,11 @@ struct PrefixArgs {
 // what holds the rows' operands and sums in registers at two waves per SIMD
 constexpr bool prefix_dim(int d) { return d % 64 == 0; }
 constexpr int prefix_columns(int d) { return d <= 128 ? 4 : 2; }
+// Workgroups per CU (one wave of each per SIMD) of an instance: few rows need few
+// registers and wait for memory
+constexpr int prefix_waves(int d, int nc, bool res) {
+    return nc == 1 && d <= 128 ? (res ? 3 : 4) : !res && d <= 128 && nc == 2 ? 3 : 2;
+}
 // nc 1, 2 or 4 (at most prefix_columns): 16 nc rows per workgroup; grid.x splits,
 // grid.y kv heads times groups of rows
 template <int D>

@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t as_u(h2_t h) { return __builtin_bit_cast(uin
 __device__ __forceinline__ uint32_t fp4_signs(uint32_t w, int p) { return ((w << (3 - p)) & 0x88888888u) | 0x22222222u; }
 
 template <int D, int NC, bool RES>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bc::prefix_waves(D, NC, RES), bc::prefix_waves(D, NC, RES))))
 void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
     constexpr int SB = D / 8, CB = D / 2, NB = D / 16, W = D / 32, NS = (D + 127) / 128;
     constexpr int Q = D / 32;    // 16-byte pieces per code row
@@ -68,7 +68,12 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
     constexpr int kQ = NC * (W + NS) * 1024;
     constexpr int RS = D + 1;                                 // row of the sums at the end
     constexpr int kLoop = QL ? 2 * kP + kQ : 2 * kP;
-    constexpr int kBuf = (kLoop > kQ ? kLoop : kQ) > R * RS * 4 ? (kLoop > kQ ? kLoop : kQ) : R * RS * 4;
+    constexpr int kRaw = 4 * NC * ((D + 127) / 128) * 1024;   // the rows as they came
+    constexpr bool kRawIn = QL && NC * NS * 1024 + kRaw <= 2 * kP;   // in the weights' place
+    constexpr int kRawAt = kRawIn ? NC * NS * 1024 : QL ? 2 * kP + kQ : kQ;
+    constexpr int kStart = kRawIn ? 2 * kP + kQ : kRawAt + kRaw;
+    constexpr int kEnd = R * RS * 4;
+    constexpr int kBuf = ((kLoop > kStart ? kLoop : kStart) > kEnd ? (kLoop > kStart ? kLoop : kStart) : kEnd) + 15 & ~15;
     __shared__ __attribute__((aligned(16))) uint8_t stage0[kCodeBytes + kSignBytes];
     __shared__ __attribute__((aligned(16))) uint8_t stage1[kCodeBytes + kSignBytes];
     __shared__ __attribute__((aligned(16))) uint8_t buf[kBuf];
@@ -200,6 +205,10 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
     load_k(k_odd, 1);
     // (past the weights' buffers where it stays, else past the sign words, in their place)
     uint8_t* const q_lds = buf + (QL ? 2 * kP : NC * NS * 1024);
+    // (the rows wait in LDS: the loops over them stay rolled, since straight-line code
+    // that runs once is fetched for as long as it takes)
+    bc_v4u* const q_raw = (bc_v4u*)(buf + kRawAt) + wave * (NC * N * 64);
+    float top = 0.0f;
     auto row16 = [](float t, auto op) {
         t = op(t, dpp_f<0x128>(t));
         t = op(t, dpp_f<0x124>(t));
@@ -209,16 +218,31 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
     // (the type by a mask: a choice per element became a branch per element)
     const uint32_t bf = a.bf16 ? 0xFFFFFFFFu : 0u;
     auto value = [&](const bc_v4u& w, int e) { return bc::half_f((uint16_t)(w[e >> 1] >> (16 * (e & 1))), bf); };
-    float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < NC; i++)
 #pragma unroll
         for (int k = 0; k < N; k++)
+            if (lj + 16 * k < D / 8) q_raw[(i * N + k) * 64 + lane] = raw[i][k];
+    // limits of the rows (those past the batch and those of a bad length, whose sums
+    // nobody reads, mask nothing)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float t = fabsf(value(raw[i][k], e));
-                top = fmaxf(top, t < INFINITY ? t : 0.0f);
-            }
+    for (int i = 0; i < NC; i++) {
+        const int r = 4 * (wave + 4 * i) + g4;
+        if (lj == 0) ((int*)row_const[r])[2] = !live[i] || bc::paged_bad_len(a, len[i]) ? 0x7FFFFFFF : len[i];
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll 1
+    for (int i = 0; i < NC * N; i++) {
+        if (lj + 16 * (i % N) >= D / 8) continue;
+        const bc_v4u w = q_raw[i * 64 + lane];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float t = fabsf(value(w, e));
+            top = fmaxf(top, t < INFINITY ? t : 0.0f);
+        }
+    }
     top = wave_max(top);
     if (lane == 0) qtop[wave] = top;
     for (int i = threadIdx.x; i < 4 * R; i += 256) (&rmax[0][0])[i] = -INFINITY;
@@ -231,46 +255,44 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
     const int ex = __builtin_amdgcn_readfirstlane(field > 0 ? 140 - field : 0);
     const float isd2 = kLog2e / sqrtf((float)D);
     const float res_unit = ldexpf(isd2 * (1.0f / 7.0f), 24 - ex);
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < NC; i++) {
         const int r = 4 * (wave + 4 * i) + g4, c = r >> 4, col = r & 15;
         float sum = 0.0f, total = 0.0f;
 #pragma unroll
         for (int k = 0; k < N; k++) {
             const int u = lj + 16 * k;
+            if (u >= D / 8) continue;
+            const bc_v4u w = q_raw[(i * N + k) * 64 + lane];
             uint32_t byte = 0;
             float t[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float v = value(raw[i][k], e);
+                const float v = value(w, e);
                 byte |= (v >= 0.0f ? 0u : 1u) << e;
                 sum += fabsf(v);
                 t[e] = ldexpf(v, ex);
                 total += t[e];
             }
-            if (u < D / 8) {
-                const int g = u / W, s = u % W;
-                if constexpr (RES) {
-                    // slots of a step: dims 0, 4, 1, 5, 2, 6, 3, 7
-                    uint32_t w[4];
+            const int g = u / W, s = u % W;
+            if constexpr (RES) {
+                // slots of a step: dims 0, 4, 1, 5, 2, 6, 3, 7
+                uint32_t h[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float f = e & 1 ? 0.0625f : 1.0f;
-                        w[e] = (uint32_t)f2h(t[e] * f) | ((uint32_t)f2h(t[e + 4] * f) << 16);
-                    }
-                    *(v4u_t*)(q_lds + ((c * W + s) * 64 + 16 * g + col) * 16) = v4u_t{w[0], w[1], w[2], w[3]};
+                for (int e = 0; e < 4; e++) {
+                    const float f = e & 1 ? 0.0625f : 1.0f;
+                    h[e] = (uint32_t)f2h(t[e] * f) | ((uint32_t)f2h(t[e + 4] * f) << 16);
                 }
-                // sign word u / 4 of the row, byte u % 4 (expanded when it is read)
-                buf[((c * NS + u / 16) * 64 + 16 * (u / 4 % 4) + col) * 16 + u % 4] = (uint8_t)byte;
+                *(v4u_t*)(q_lds + ((c * W + s) * 64 + 16 * g + col) * 16) = v4u_t{h[0], h[1], h[2], h[3]};
             }
+            // sign word u / 4 of the row, byte u % 4 (expanded when it is read)
+            buf[((c * NS + u / 16) * 64 + 16 * (u / 4 % 4) + col) * 16 + u % 4] = (uint8_t)byte;
         }
         sum = row16(sum, [](float p, float q) { return p + q; });
         total = row16(total, [](float p, float q) { return p + q; });
         if (lj == 0) {
             row_const[r][0] = sum * (1.0f / (float)D) * isd2;
             row_const[r][1] = ldexpf(-8.0f * total, -24);
-            // (padding rows and rows of a bad length, whose sums nobody reads, mask nothing)
-            ((int*)row_const[r])[2] = !live[i] || bc::paged_bad_len(a, len[i]) ? 0x7FFFFFFF : len[i];
         }
     }
     lds_barrier();
@@ -413,15 +435,14 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
                 const float sum = (p[0] + p[1]) + (p[2] + p[3]);
                 sums[c] = sum;
                 // weights as operands: keys (j = 0, 1) and (2, 3) of the lane share a dword
-                h2_t w0, w1;
-                w0[0] = (_Float16)(p[0] * fa[0]); w0[1] = (_Float16)(p[1] * fa[1]);
-                w1[0] = (_Float16)(p[2] * fa[2]); w1[1] = (_Float16)(p[3] * fa[3]);
-                v2u_t wa = {as_u(w0), as_u(w1)}, wb = {0u, 0u};
-                if constexpr (RES) {
-                    w0[0] = (_Float16)(p[0] * fb[0]); w0[1] = (_Float16)(p[1] * fb[1]);
-                    w1[0] = (_Float16)(p[2] * fb[2]); w1[1] = (_Float16)(p[3] * fb[3]);
-                    wb = v2u_t{as_u(w0), as_u(w1)};
-                }
+                auto weights = [&](const f4_t& f) {
+                    h2_t w0, w1;
+                    w0[0] = (_Float16)(p[0] * f[0]); w0[1] = (_Float16)(p[1] * f[1]);
+                    w1[0] = (_Float16)(p[2] * f[2]); w1[1] = (_Float16)(p[3] * f[3]);
+                    return v2u_t{as_u(w0), as_u(w1)};
+                };
+                v2u_t wa = weights(fa), wb = {0u, 0u};
+                if constexpr (RES) wb = weights(fb);
                 if (!whole) {
                     // (a masked key adds nothing whatever its scales are)
 #pragma unroll
@@ -542,8 +563,9 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
                 const int p = (block0 + i) & 3;
 #pragma unroll
                 for (int mh = 0; mh < 2; mh++) {
-                    // the sign bit from the value's bit p
-                    const uint32_t v = ~(uint32_t)(mh ? bits[i].y : bits[i].x);
+                    // the sign bit is the value's bit p (so -1 where the value is positive:
+                    // turned at the end)
+                    const uint32_t v = (uint32_t)(mh ? bits[i].y : bits[i].x);
                     uint32_t u[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++) u[j] = ((v << (15 - 4 * j - p)) & 0x80008000u) | 0x3C003C00u;
@@ -577,7 +599,7 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
 #pragma unroll
         for (int i = 0; i < NBW; i++) {
             const int b = block0 + i, p = b & 3;
-            const float k = res ? unit * (1.0f / 7.0f) : unit;
+            const float k = res ? unit * (1.0f / 7.0f) : -unit;
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -595,12 +617,18 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
         if (res_wave) put(true);
         __syncthreads();
     }
-    // (a wave a row: its place is scalar arithmetic)
-    for (int r = wave; r < R; r += 4) {
-        const int row = row0 + r;
-        if (row >= rows) break;
-        const int b = row / group, h = hkv * group + row - b * group;
-        float* const dst = x.ws + (((int64_t)blockIdx.x * a.B + b) * a.Hq + h) * (D + 2);
+    // (a wave a row; where row r goes in lane r)
+    int64_t place_of = 0;
+    if (lane < R && row0 + lane < rows) {
+        const int b = (row0 + lane) / group, h = hkv * group + (row0 + lane) - b * group;
+        place_of = (((int64_t)blockIdx.x * a.B + b) * a.Hq + h) * (D + 2);
+    }
+    const int last_row = min(R, rows - row0);
+#pragma unroll 4
+    for (int r = wave; r < last_row; r += 4) {
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)place_of, r);
+        const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)place_of >> 32), r);
+        float* const dst = x.ws + (int64_t)((uint64_t)hi << 32 | lo);
 #pragma unroll
         for (int e = 0; e < D; e += 64) dst[2 + e + lane] = o[r * RS + e + lane];
         if (lane == 0) {
