@@ -266,3 +266,38 @@ def test_refusals(F):
     bad(pa, k, v, slots, blobs[0], blobs[1], blobs[2], None, 64)
     bad(pa, k, v, slots, blobs[0], torch.zeros(130 * 64, dtype=torch.uint8, device="cuda"), blobs[2], blobs[3], 64)
     bad(pa, k, v, slots, blobs[0].cpu(), blobs[1], blobs[2], blobs[3], 64)
+
+
+LANES = [(d, rot, dtype) for d, dtype in ((32, torch.float16), (64, torch.bfloat16), (96, torch.float16),
+                                          (128, torch.bfloat16), (160, torch.float16), (224, torch.bfloat16),
+                                          (256, torch.float16))
+         for rot in (16, 32, 64) if rot <= d]
+
+
+@pytest.mark.parametrize("d,rot,dtype", LANES, ids=[f"{d}-{r}" for d, r, _ in LANES])
+def test_few_turned_dims(F, d, rot, dtype):
+    """Half pairs within the first 64 elements, with norms and without; the elements past
+    them, infinities and signs of zero among them, stay where there is no norm."""
+    s = inputs(d + rot, 11, 3, 2, d, rot, dtype, True)
+    q, k = F.norm_rotary(s["q"], s["k"], s["pos"], s["cos"], s["sin"], k_weight=s["wk"])
+    assert_rows(q, reference(s["q"], s, None, 1e-6, False))
+    assert_rows(k, reference(s["k"], s, s["wk"], 1e-6, False))
+    if rot < d:
+        x = s["q"].clone()
+        x[0, 0, rot], x[1, 0, d - 1], x[2, 1, rot] = float("inf"), float("-inf"), -0.0
+        q, _ = F.norm_rotary(x, None, s["pos"], s["cos"], s["sin"])
+        assert torch.equal(q[..., rot:].contiguous().view(torch.int16), x[..., rot:].contiguous().view(torch.int16))
+
+
+@pytest.mark.parametrize("d,inter,layout", [(128, False, "fused"), (96, True, "whole"), (96, False, "odd")])
+def test_long_prompt_is_its_parts(F, d, inter, layout):
+    """Rows past what the caches hold are read by other loads: the same rows."""
+    T = 45000
+    s = inputs(2, T, 9, 1, d, d, torch.bfloat16, True, layout)
+    s["pos"] = torch.arange(T, device="cuda") % s["cos"].shape[0]
+    call = lambda a, b: F.norm_rotary(s["q"][a:b], s["k"][a:b], s["pos"][a:b], s["cos"], s["sin"], q_weight=s["wq"],
+                                      k_weight=s["wk"], interleaved=inter)
+    q, k = call(0, T)
+    for a, b in ((0, 9001), (9001, 20000), (20000, 31111), (31111, T)):
+        qp, kp = call(a, b)
+        assert torch.equal(q[a:b], qp) and torch.equal(k[a:b], kp)
