@@ -21,11 +21,12 @@
 // under them, and nothing that they need is held in 64 bits over the rows (104
 // registers in place of 212: 80 us against 92).
 //
-// 16384 tokens of 32 and 8 heads of 128 (bf16, 344 MB): 63 us, 5.4 TB/s, what a
-// copy of as many bytes takes; 5001 of 64 heads of 96, a third of them turned
-// (fp16, 124 MB): 30 us, 4.1 TB/s; 4 tokens 5.4 us.  With the append: 16383 tokens
+// 16384 tokens of 32 and 8 heads of 128 (bf16, 344 MB): 68 us, 5.0 TB/s, where a
+// copy of as many bytes takes 65; 5001 of 64 heads of 96, a third of them turned
+// (fp16, 124 MB): 29 us, 4.3 TB/s; 4 tokens 5.4 us.  With the append: 16383 tokens
 // (bf16, 366 MB) 80 us, 4.6 TB/s; signs of 4096 tokens of 3 x 32 heads of 64 (fp16,
-// 71 MB) 19 us, 3.7 TB/s; 32 tokens 5.4 us.
+// 71 MB) 17 us, 4.2 TB/s; 32 tokens 5.4 us.  Half pairs read again (PAIR_ROW) cost
+// their conversions twice: 16384 tokens of 64 heads of 96 124 us, 86 in neighbours.
 #include <math.h>
 
 #include "common.h"
@@ -56,8 +57,10 @@ struct RotaryArgs {
     const int64_t* slots;      // [T]
     int64_t n_slots;
     FastDiv page;              // slots per page
+    FastDiv inner;             // workgroups are (outer, inner) of token blocks and head groups
     double eps;
     int T, R, total_heads, heads_per_wave, kv_heads;
+    int heads_first;           // inner is the head group
 };
 
 // How a lane finds the partner of an element: in its own slices (half pairs of
@@ -159,7 +162,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     constexpr int NE = PAIR == PAIR_NEXT ? 4 : 8;             // ... and factors of a slice
     const int lane = threadIdx.x & 63, sub = lane >> 3, j = lane & 7;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t first = ((int64_t)blockIdx.x * (blockDim.x >> 6) + wave) * 8;
+    const uint32_t outer = bc::fast_div(blockIdx.x, a.inner), inner = blockIdx.x - outer * a.inner.d;
+    const uint32_t block = a.heads_first ? outer : inner, group = a.heads_first ? inner : outer;
+    const int64_t first = ((int64_t)block * (blockDim.x >> 6) + wave) * 8;
     if (first >= a.T) return;
     const bool token_live = first + sub < a.T;
     const int64_t t = token_live ? first + sub : a.T - 1;
@@ -197,7 +202,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         offset = (int)(u - (uint32_t)page * a.page.d);
     }
 
-    const int h_first = blockIdx.y * a.heads_per_wave;
+    const int h_first = (int)group * a.heads_per_wave;
     const int h_last = min(a.total_heads, h_first + a.heads_per_wave);
     int base = 0;
 #pragma unroll 1
@@ -217,7 +222,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         bc_v4u next[K], nextp[PAIR == PAIR_ROW ? K : 1];
         // (a builtin of its own where the rows are read past the caches: of two plain loads
         // the compiler would make one)
-        const __amdgpu_buffer_rsrc_t block = __builtin_amdgcn_make_buffer_rsrc(
+        const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(
             (void*)(P.src + first * P.token_stride), (short)0, INT32_MAX, 0x00020000);
         const int mine = (int)(t - first) * (int)P.token_stride * 2 + 16 * j;
         const bool stream = P.stream != 0;
@@ -227,7 +232,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
                 const int at = h * (int)P.head_stride * 2;
 #pragma unroll
                 for (int k = 0; k < K; k++)
-                    next[k] = __builtin_amdgcn_raw_buffer_load_b128(block, inside(k) ? mine + 128 * k : INT32_MAX, at, 2);
+                    next[k] = __builtin_amdgcn_raw_buffer_load_b128(rows, inside(k) ? mine + 128 * k : INT32_MAX, at, 2);
             } else {
 #pragma unroll
                 for (int k = 0; k < K; k++) next[k] = load_eight(x0 + (inside(k) ? 64 * k + 8 * j : 0));
@@ -459,26 +464,34 @@ int launch(RotaryArgs& a, int head_dim, int interleaved, int dtype, hipStream_t 
                      : head_dim % 128 == 0 && (a.R == head_dim || a.R == 0) ? PAIR_OWN
                      : a.R == 64 || a.R == 32 || a.R == 16 || a.R == 0      ? PAIR_LANE
                                                                             : PAIR_ROW;
-    // Rows that the caches cannot hold are read past them, which leaves them to the
-    // outputs: 168 MB of rows (344 MB in and out) 80 us and 62.  Fewer, just written or
-    // soon read again, are better left there: 25 to 63 MB 1 to 2 us less of 14 to 30.
-    // (Offsets within a wave's eight tokens are 31 bits.)
+    // Rows that the caches cannot hold: read past them, which leaves them to the outputs,
+    // and in the order of their addresses, all heads of a block of tokens beside each
+    // other and few heads a wave, so that the workgroups of a moment lie close together
+    // in memory: 16384 tokens of 40 heads of 128 86 us without either, 84 read past the
+    // caches, 68 in order too; with the append 102 and 80.  Fewer rows, just written or
+    // soon read again, are better left there (25 to 63 MB 1 to 2 us less of 14 to 30),
+    // and more heads a wave then share its factors (4096 tokens of 96 heads of 64,
+    // appended: 16.6 us, 20.7 in order).
     constexpr int64_t kStreamBytes = 80 << 20;
     int64_t bytes = 0;
     for (const RotaryRows& r : a.rows) bytes += (int64_t)a.T * r.heads * head_dim * 2;
+    const bool stream = bytes > kStreamBytes;
+    // (offsets within a wave's eight tokens are 31 bits)
     for (RotaryRows& r : a.rows) {
         const int64_t ts = r.token_stride * 2, hs = r.head_stride * 2, limit = 1 << 27;
-        r.stream = bytes > kStreamBytes && ((uintptr_t)r.src | (uint64_t)ts | (uint64_t)hs) % 16 == 0 && ts >= 0 &&
-                   ts < limit && hs >= 0 && hs < limit && hs * r.heads < 1 << 30;
+        r.stream = stream && ((uintptr_t)r.src | (uint64_t)ts | (uint64_t)hs) % 16 == 0 && ts >= 0 && ts < limit &&
+                   hs >= 0 && hs < limit && hs * r.heads < 1 << 30;
     }
-    // heads of a wave: all, or as few as give every CU 24 waves (the prompt's append: 16
-    // waves 80 us, 24 and 32 79 to 82; 4096 tokens, heads of 64: 22, 20 and 22)
+    // heads of a wave: all, or as few as give every CU 24 waves (40; 32 and 48 2 us more)
     const int64_t octets = ((int64_t)a.T + 7) / 8, blocks = (octets + 3) / 4;
-    const int64_t want = 24LL * bc::device_cu_count();
+    const int64_t want = (int64_t)(stream ? 40 : 24) * bc::device_cu_count();
     int64_t groups = (want + octets - 1) / octets;
     if (groups > a.total_heads) groups = a.total_heads;
     a.heads_per_wave = (int)((a.total_heads + groups - 1) / groups);
-    const dim3 grid((unsigned)blocks, (a.total_heads + a.heads_per_wave - 1) / a.heads_per_wave);
+    groups = (a.total_heads + a.heads_per_wave - 1) / a.heads_per_wave;
+    a.heads_first = stream;
+    a.inner = bc::make_fastdiv((uint32_t)(stream ? groups : blocks));
+    const dim3 grid((unsigned)(blocks * groups));
 #define BC_CASE(DD)                                                        \
     case DD:                                                               \
         if (dtype == BC_BF16) launch_rotary<DD, true>(a, pair, grid, st);  \
