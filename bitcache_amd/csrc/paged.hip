@@ -2,6 +2,7 @@
 // and merge.  The attention itself is attn_mfma_kernel.h's paged instances over
 // work units that the device cuts from the lengths (attn.h, PagedUnit).
 #include <math.h>
+#include <stdlib.h>
 
 #include "attn.h"
 #include "prefix_attn.h"
@@ -117,10 +118,23 @@ struct PagedPlan {
     size_t own_bytes, bytes;   // of the units' partials, and with the prefix's
 };
 
-// The shared prefix: groups of 16 nc query rows, and as many workgroups as the CUs hold.
+// Whether the shared prefix has its own kernel: where the sequences would read 192 MB
+// or more of it.  Less, and its launch and its partials cost more than the bytes
+// (whole calls, 200 keys more per sequence, us without and with it; residual
+// planes, 32/8 heads of 128: 32768 keys, 4 sequences 38 and 42, 8 52 and 45, 32 140
+// and 77; 8192 keys, 16 sequences 36 and 43, 32 50 and 52; 32/32 heads, 2048 keys, 8
+// sequences 24 and 25, 32 57 and 40; signs only, 32/8 heads, 32768 keys, 16
+// sequences 40 and 48, 32 61 and 58).  BITCACHE_SHARED=1 and =0 choose it always and never (tuning).
+bool prefix_pays(int mode, int64_t batch, int n_kv_heads, int64_t shared_len, int d) {
+    if (const char* e = getenv("BITCACHE_SHARED")) return e[0] == '1';
+    const int64_t pair = 2 * (mode == MODE_BINARY ? d / 8 + 2 : d / 8 + 2 + d / 2 + 2);
+    return batch * shared_len * n_kv_heads * pair >= 192ll << 20;
+}
+
+// Its plan: groups of 16 nc query rows, and as many workgroups as the CUs hold.
 void plan_prefix(PagedPlan& p, int mode, int batch, int n_heads, int n_kv_heads, int shared_len, int d) {
     const int64_t rows = (int64_t)batch * (n_heads / n_kv_heads);
-    if (shared_len == 0 || batch < 2 || !bc::prefix_dim(d)) return;
+    if (shared_len == 0 || batch < 2 || !bc::prefix_dim(d) || !prefix_pays(mode, batch, n_kv_heads, shared_len, d)) return;
     p.nc = rows <= 16 ? 1 : rows <= 32 ? 2 : bc::prefix_columns(d);
     p.row_groups = (int)((rows + 16 * p.nc - 1) / (16 * p.nc));
     const int tiles = shared_len / 64;

@@ -17,6 +17,12 @@ def F():
     return functional
 
 
+@pytest.fixture(autouse=True)
+def shared_kernel(monkeypatch):
+    """The shared prefix's kernel at the tests' sizes too."""
+    monkeypatch.setenv("BITCACHE_SHARED", "1")
+
+
 def rng(seed):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -350,3 +356,14 @@ def test_refusals(F):
     bad(q.clone().requires_grad_(), tables, lens)
     e = F.paged_attention(q[:0], *blobs, tables[:0], lens[:0], 256, 64, n_kv_heads=2)
     assert e.shape == (0, 8, 128)
+
+
+@pytest.mark.parametrize("residual,B", [(True, 24), (False, 2), (True, 2)])
+def test_shared_prefix_by_its_size(F, monkeypatch, residual, B):
+    """The rule's own choice, and both ways by force: each within the bound."""
+    own = [1 + 37 * i for i in range(B)]
+    lens = [2560 + n for n in own]
+    q, blobs, tables, lens_t = setup(40 + B, lens, 16, 16, 256, 64, residual, torch.bfloat16, shared=2560)
+    for choice in (None, "0", "1"):
+        monkeypatch.delenv("BITCACHE_SHARED") if choice is None else monkeypatch.setenv("BITCACHE_SHARED", choice)
+        check(F, q, blobs, tables, lens_t, 64, 16, max(lens), shared=2560, what=f"choice {choice}")
