@@ -55,6 +55,7 @@ struct AttnArgs {
     int width, n_pages, page_tiles, key0, max_len;
     int unit_tiles;   // see PagedUnit; 0: one unit per sequence
     int unit_slots, unit_most;
+    int2* units;      // each sequence's first unit and how many it has
     int bf16;         // queries and outputs are bf16
 };
 
@@ -133,15 +134,26 @@ __device__ __forceinline__ int paged_chunk(const AttnArgs& a, int lane, int& own
     uint32_t cost[1] = {~((uint32_t)fminf(16.0f * tiles, 268435455.0f) << 3 | (uint32_t)cand)};
     if (units > a.unit_most) cost[0] = 0;
     wave_umax(cost);
-    return cost[0] == 0 ? kUnitTiles : __builtin_amdgcn_readlane(chunk, (int)(~cost[0] & 7));
+    const uint32_t best = __builtin_amdgcn_readfirstlane(cost[0]);
+    return best == 0 ? kUnitTiles : __builtin_amdgcn_readlane(chunk, (int)(~best & 7));
 }
-__device__ __forceinline__ PagedUnit paged_unit(const AttnArgs& a, int unit, int lane) {
+// tells: the caller is the wave that notes every sequence's units (with unit 0)
+__device__ __forceinline__ PagedUnit paged_unit(const AttnArgs& a, int unit, int lane, bool tells) {
     if (a.unit_tiles == 0) {
         const int len = __builtin_amdgcn_readfirstlane(a.lens[unit]);
         return PagedUnit{unit, len, 0, paged_tiles(a, len)};
     }
     int own;
     const int chunk = paged_chunk(a, lane, own);
+    if (unit == 0 && tells) {
+        int base = 0;
+        for (int i0 = 0; i0 < a.B; i0 += 64) {
+            const int tiles = i0 == 0 ? own : i0 + lane < a.B ? paged_tiles(a, a.lens[i0 + lane]) : 0;
+            const int n = (tiles + chunk - 1) / chunk, incl = wave_scan_add(n);
+            if (i0 + lane < a.B) a.units[i0 + lane] = make_int2(base + incl - n, n);
+            base += __builtin_amdgcn_readlane(incl, 63);
+        }
+    }
     int base = 0;
     for (int i0 = 0; i0 < a.B; i0 += 64) {
         const int tiles = i0 == 0 ? own : i0 + lane < a.B ? paged_tiles(a, a.lens[i0 + lane]) : 0;
@@ -158,26 +170,6 @@ __device__ __forceinline__ PagedUnit paged_unit(const AttnArgs& a, int unit, int
     }
     return PagedUnit{-1, 0, 0, 0};
 }
-// The first unit of sequence b, and how many it has
-struct PagedUnits {
-    int first, count;
-};
-__device__ __forceinline__ PagedUnits paged_units(const AttnArgs& a, int b, int lane) {
-    int own;
-    const int chunk = paged_chunk(a, lane, own);
-    int base = 0;
-    for (int i0 = 0;; i0 += 64) {
-        const int tiles = i0 == 0 ? own : i0 + lane < a.B ? paged_tiles(a, a.lens[i0 + lane]) : 0;
-        const int n = (tiles + chunk - 1) / chunk;
-        const int incl = wave_scan_add(n);
-        if (b < i0 + 64) {
-            const int count = __builtin_amdgcn_readlane(n, b - i0);
-            return PagedUnits{base + __builtin_amdgcn_readlane(incl, b - i0) - count, count};
-        }
-        base += __builtin_amdgcn_readlane(incl, 63);
-    }
-}
-
 // Packs per row of the stored popcounts: S rounded up to 16, so that every
 // row starts 16-byte aligned and eight-key runs load whole.
 __host__ __device__ inline int pcs_stride(int S) { return (S + 15) & ~15; }

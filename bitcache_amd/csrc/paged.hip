@@ -23,7 +23,7 @@ using bc::MODE_COMP;
 // The merge of a sequence's units, and of the shared prefix's `splits` partials per
 // row: PARTS waves per (sequence, query head), each over every PARTS-th partial
 // (lane = partial for the factors, lanes = dims for the sums), joined in LDS.
-// Bound: the latency of its three loads in turn (lengths, maxima, sums).
+// Bound: the latency of its three loads in turn (units, maxima, sums).
 template <int D, int PARTS>
 __global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t* out, const float* prefix, int splits) {
     constexpr int N = (D + 63) / 64;     // dims of a lane
@@ -34,11 +34,13 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t
     const int64_t row = (int64_t)blockIdx.x * ROWS + wave / PARTS;
     const bool live = row < (int64_t)a.B * a.Hq;
     const int b = live ? (int)(row / a.Hq) : 0, h = live ? (int)(row - (int64_t)b * a.Hq) : 0;
-    const bc::PagedUnits u = bc::paged_units(a, b, lane);
+    // (without units: all keys are the prefix's)
+    const int2 u = a.unit_most > 0 ? a.units[b] : make_int2(0, 0);
+    const int len = a.lens[b];
     const int64_t own_step = (int64_t)a.Hq * (D + 2), prefix_step = own_step * a.B;
-    const float* const own = a.ws + (int64_t)u.first * own_step + (int64_t)h * (D + 2);
+    const float* const own = a.ws + (int64_t)u.x * own_step + (int64_t)h * (D + 2);
     const float* const shared = prefix + ((int64_t)b * a.Hq + h) * (D + 2);
-    const int total = live ? splits + u.count : 0;
+    const int total = live ? splits + u.y : 0;
     // (s-th partial of this wave)
     auto partial = [&](int s) {
         s = s * PARTS + part;
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t
         }
     }
     if (!live) return;
-    const bool bad = bc::paged_bad_len(a, a.lens[b]);   // (NaN where the length is out of bounds)
+    const bool bad = bc::paged_bad_len(a, len);   // (NaN where the length is out of bounds)
     const float inv = bad ? __builtin_nanf("") : L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
     for (int n = 0; n < N; n++)
@@ -115,8 +117,11 @@ struct PagedPlan {
     int units;         // at most
     // the shared prefix's kernel (splits 0: the prefix is attended as own keys)
     int splits, tiles_per, nc, row_groups;
-    size_t own_bytes, bytes;   // of the units' partials, and with the prefix's
+    size_t own_bytes, bytes;   // of the units' notes and partials, and with the prefix's
 };
+
+// What notes every sequence's units
+size_t note_bytes(int batch) { return ((size_t)batch * sizeof(int2) + 15) & ~(size_t)15; }
 
 // Whether the shared prefix has its own kernel: where the sequences would read 192 MB
 // or more of it.  Less, and its launch and its partials cost more than the bytes
@@ -168,7 +173,7 @@ PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len
     int64_t units = bc::paged_unit_most(p.unit_slots, batch, batch * tiles);
     if (units > most) units = most;
     p.units = (int)units;
-    p.own_bytes = (size_t)units * n_heads * (d + 2) * sizeof(float);
+    p.own_bytes = note_bytes(batch) + (size_t)units * n_heads * (d + 2) * sizeof(float);
     p.bytes = p.own_bytes + (size_t)p.splits * batch * n_heads * (d + 2) * sizeof(float);
     return p;
 }
@@ -246,7 +251,7 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     a.B = batch;
     a.Hq = n_heads;
     a.Hkv = n_kv_heads;
-    a.ws = (float*)workspace;
+    a.ws = (float*)((uint8_t*)workspace + note_bytes(batch));
     a.lens = seq_lens;
     a.tables = block_tables;
     a.width = table_width;
@@ -256,6 +261,8 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     a.unit_tiles = p.unit_tiles;
     a.unit_slots = p.unit_slots;
     a.unit_most = p.units;
+    // (the workspace: the sequences' units, their partials, the prefix's)
+    a.units = (int2*)workspace;
     a.bf16 = dtype == BC_BF16;
     float* const prefix_ws = (float*)((uint8_t*)workspace + p.own_bytes);
     // (a pool without pages holds no length but zero: nothing to attend)
