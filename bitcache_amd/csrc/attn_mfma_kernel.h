@@ -741,27 +741,30 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
     // pieces swizzled as above) or piece c at c*1024 + 16k (per key)
     auto issue_v = [&](int buf, int t0) {
         const int tr = PG ? 0 : t0 - key_begin;
+        // (paged: the same offsets every tile, made anew: held, they spill, and a reload waits
+        // for every load in flight)
+        const int ln = PG ? opaque_int(lane) : lane;
         const __amdgpu_buffer_rsrc_t r_vst = at_tile(r_vs, v_signs, SB, t0);
         uint8_t* st_codes = buf ? lds_st1[wave] : lds_st0[wave];
         uint8_t* st_signs = st_codes + WL::kCodeBytes;
         if constexpr (WL::kSignPad) {
             // a dword per lane: RW lanes per row, 64 / RW rows per load
             constexpr int RW = WL::kSignStride / 4;
-            const int w = min(lane % RW, SB / 4 - 1);
+            const int w = min(ln % RW, SB / 4 - 1);
 #pragma unroll
             for (int c = 0; c < RW; c++)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vst, LDS_PTR(void, st_signs + c * 256), 4,
-                                                         (tr + c * (64 / RW) + lane / RW) * SB + 4 * w, 0, 0, 0);
+                                                         (tr + c * (64 / RW) + ln / RW) * SB + 4 * w, 0, 0, 0);
         } else {
             // whole KiB, and a half one at d = 64 and 192 (whose lanes 32..63
             // repeat lanes 0..31 into the half past the rows)
 #pragma unroll
             for (int c = 0; c < SB / 16; c++)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vst, LDS_PTR(void, st_signs + c * 1024), 16,
-                                                         tr * SB + 16 * lane + c * 1024, 0, 0, BC_NT_AUX);
+                                                         tr * SB + 16 * ln + c * 1024, 0, 0, BC_NT_AUX);
             if constexpr (SB % 16 != 0)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(r_vst, LDS_PTR(void, st_signs + SB / 16 * 1024), 16,
-                                                         tr * SB + 16 * (lane & 31) + SB / 16 * 1024, 0, 0, 0);
+                                                         tr * SB + 16 * (ln & 31) + SB / 16 * 1024, 0, 0, 0);
         }
         if constexpr (ALLRES) {
             const __amdgpu_buffer_rsrc_t r_vct = at_tile(r_vc, v_codes, CB, t0);
@@ -769,8 +772,8 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
             for (int c = 0; c < Q; c++)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     r_vct, LDS_PTR(void, st_codes + c * 1024), 16,
-                    LIN_V ? tr * CB + c * 1024 + 16 * (Q_POW2 ? lane ^ ((4 * c + (lane >> 4)) & (Q - 1)) : lane)
-                          : (tr + lane) * CB + 16 * c, 0, 0, LIN_V ? BC_NT_AUX : 0);
+                    LIN_V ? tr * CB + c * 1024 + 16 * (Q_POW2 ? ln ^ ((4 * c + (ln >> 4)) & (Q - 1)) : ln)
+                          : (tr + ln) * CB + 16 * c, 0, 0, LIN_V ? BC_NT_AUX : 0);
         }
     };
 
