@@ -69,10 +69,11 @@ struct AttnArgs {
 // tiles), as far as its units fit the launched ones (unit_most); chunk is at
 // least unit_tiles and at most kUnitTiles (a wave holds its tiles' places in one
 // register), which always fits.  unit_tiles = 0: unit b is sequence b.  Each wave
-// finds its unit by itself.  (64 sequences of 128 to 32768 keys, 32/8 heads: 119
+// finds its unit by itself, and one notes the sequences' units for the merge.  (64
+// sequences of 128 to 32768 keys, 32/8 heads, by an earlier form of the kernel: 119
 // us; the candidates taken alone 112 to 124, those that do not fit 180; one equal
-// range of tiles per slot, across sequences, 159: two segments in most ranges,
-// each with the fixed work and none beside another's loop.)
+// range of tiles per slot, across sequences, 159: two segments in most ranges, each
+// with the fixed work and none beside another's loop.)
 constexpr int kUnitTiles = 256, kUnitFixed = 4, kUnitRounds = 2;
 struct PagedUnit {
     int b, len;        // (b < 0: no such unit)
