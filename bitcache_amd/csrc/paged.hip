@@ -237,6 +237,9 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     if ((int64_t)batch * n_heads == 0) return BC_OK;
     BC_REQUIRE(q && out && seq_lens && (table_width == 0 || block_tables) && (n_pages == 0 || (k_bin && v_bin)),
                BC_ERR_INVALID_ARGUMENT, "null pointer");
+    // (planes start where their vectors are whole 16 bytes, after 64 and more of them)
+    BC_REQUIRE((((uintptr_t)k_bin | (uintptr_t)k_res | (uintptr_t)v_bin | (uintptr_t)v_res | (uintptr_t)workspace) & 15) == 0,
+               BC_ERR_INVALID_ARGUMENT, "blobs and workspace must be 16-byte aligned");
     const int mode = k_res ? MODE_COMP : MODE_BINARY;
     const PagedPlan p = plan(mode, batch, n_heads, n_kv_heads, max_seq_len, shared_len, head_dim);
     BC_REQUIRE(p.units <= 65535, BC_ERR_UNSUPPORTED, "more than 65535 work units");

@@ -196,7 +196,9 @@ void prefix_attn_kernel(AttnArgs a, PrefixArgs x) {
 #pragma unroll
         for (int k = 0; k < N; k++) {
             raw[i][k] = bc_v4u{0u, 0u, 0u, 0u};
-            if (live[i] && lj + 16 * k < D / 8) raw[i][k] = *(const bc_v4u*)(src + 8 * (lj + 16 * k));
+            // (rows start at any element)
+            typedef uint32_t Eight __attribute__((ext_vector_type(4), aligned(2)));
+            if (live[i] && lj + 16 * k < D / 8) raw[i][k] = *(const Eight*)(src + 8 * (lj + 16 * k));
         }
     }
     place(0);

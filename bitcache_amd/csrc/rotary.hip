@@ -554,6 +554,8 @@ extern "C" int bc_paged_append(const void* q, int64_t q_token_stride, int64_t q_
     BC_REQUIRE(n_tokens == 0 || n_heads == 0 || (q && q_out), BC_ERR_INVALID_ARGUMENT, "null pointer");
     BC_REQUIRE(n_tokens == 0 || n_kv_heads == 0 || (k && v && slots && (n_pages == 0 || (k_bin && v_bin))),
                BC_ERR_INVALID_ARGUMENT, "null pointer");
+    BC_REQUIRE((((uintptr_t)k_bin | (uintptr_t)k_res | (uintptr_t)v_bin | (uintptr_t)v_res) & 15) == 0,
+               BC_ERR_INVALID_ARGUMENT, "blobs must be 16-byte aligned");
     a.slots = slots;
     a.n_slots = (int64_t)n_pages * page_size;
     a.page = bc::make_fastdiv((uint32_t)page_size);

@@ -50,9 +50,16 @@ class PagedBitCache:
 
     def slots(self, block_tables: Tensor, positions: Tensor) -> Tensor:
         """Slots [batch] int64 of position positions[b] of the sequence block_tables[b]
-        (the token a decode step appends)."""
-        page = block_tables.gather(1, (positions // self.page_size).long()[:, None])[:, 0]
-        return page.long() * self.page_size + positions.long() % self.page_size
+        (the token a decode step appends); -1, which goes nowhere, for a position outside
+        the table or on a page outside the pool."""
+        width = block_tables.shape[1]
+        if width == 0:
+            return torch.full_like(positions, -1, dtype=torch.int64)
+        positions = positions.long()
+        entry = torch.div(positions, self.page_size, rounding_mode="floor")
+        page = block_tables.gather(1, entry.clamp(0, width - 1)[:, None])[:, 0].long()
+        known = (positions >= 0) & (entry < width) & (page >= 0) & (page < self.n_pages)
+        return torch.where(known, page * self.page_size + positions % self.page_size, -1)
 
     def append(self, K: Tensor, V: Tensor, slots: Tensor) -> None:
         """Encode K, V [tokens, n_kv_heads, head_dim] into slots (functional.paged_append)."""

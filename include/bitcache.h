@@ -322,7 +322,8 @@ int bc_adaptive_attention(const void* q, const void* k_bin, const void* k_res, c
  * page_size is a multiple of 64 (the keys of an attention tile), so a tile
  * never spans two pages.  Rows of queries, keys and values are fp16 or bf16
  * (dtype), [tokens, heads, head_dim] with unit stride in the last dim and
- * strides in elements in the others (a slice of a fused projection). */
+ * strides in elements in the others (a slice of a fused projection).  Blobs,
+ * outputs of rows and workspaces are 16-byte aligned; up to 65535 heads. */
 enum bc_dtype { BC_FP16 = 0, BC_BF16 = 1 };
 
 /* Norms of query and key heads with the position rotation in the same pass:

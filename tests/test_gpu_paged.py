@@ -367,3 +367,47 @@ def test_shared_prefix_by_its_size(F, monkeypatch, residual, B):
     for choice in (None, "0", "1"):
         monkeypatch.delenv("BITCACHE_SHARED") if choice is None else monkeypatch.setenv("BITCACHE_SHARED", choice)
         check(F, q, blobs, tables, lens_t, 64, 16, max(lens), shared=2560, what=f"choice {choice}")
+
+
+def test_slots_outside_the_tables(F):
+    """Positions and pages that do not exist are padding, not an index error on the device."""
+    import bitcache_amd
+    pool = bitcache_amd.PagedBitCache(4, 64, 2, 64)
+    tables = torch.tensor([[2, 0], [-1, 3], [1, 9], [3, 1], [0, 1]], dtype=torch.int32, device="cuda")
+    at = torch.tensor([65, 3, 64, -1, 128], device="cuda")
+    assert pool.slots(tables, at).tolist() == [1, -1, -1, -1, -1]
+    assert pool.slots(tables[:, :0], at).tolist() == [-1] * 5
+    assert pool.slots(tables, torch.tensor([127, 64, 0, 63, 0], dtype=torch.int32, device="cuda")).tolist() == \
+        [63, 192, 64, 255, 0]
+
+
+@pytest.mark.parametrize("shared", [0, 640])
+def test_queries_at_odd_elements(F, shared):
+    """Contiguous queries that start at any element of their storage."""
+    lens = [641 + 50 * i for i in range(6)]
+    q, blobs, tables, lens_t = setup(50, lens, 8, 2, 128, 64, True, torch.float16, shared=shared)
+    odd = torch.empty(q.numel() + 3, dtype=q.dtype, device="cuda")[3:].view(q.shape)
+    odd.copy_(q)
+    check(F, odd, blobs, tables, lens_t, 64, 2, max(lens), shared=shared)
+    with pytest.raises(RuntimeError, match="aligned"):
+        moved = torch.empty(blobs[0].numel() + 4, dtype=torch.uint8, device="cuda")[4:]
+        F.paged_attention(q, moved, *blobs[1:], tables, lens_t, max(lens), 64, n_kv_heads=2, shared_len=shared)
+
+
+def test_two_streams_at_once(F):
+    """Calls on two streams, each with its own workspace, and the same calls alone."""
+    calls = []
+    for seed in (60, 61):
+        lens = [100 + 333 * i for i in range(20)]
+        q, blobs, tables, lens_t = setup(seed, lens, 8, 2, 128, 64, True, torch.float16)
+        calls.append(lambda q=q, b=blobs, t=tables, n=lens_t: F.paged_attention(q, *b, t, n, 7000, 64, n_kv_heads=2))
+    alone = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(c())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(alone, got))

@@ -31,6 +31,8 @@ def test_rotary_argument_errors(lib, no_gpu):  # noqa: F811
     assert call(H=-1) == BC_ERR_INVALID_ARGUMENT
     assert call(q=None) == BC_ERR_INVALID_ARGUMENT
     assert call(ko=None) == BC_ERR_INVALID_ARGUMENT
+    assert call(ko=P(0x1002)) == BC_ERR_INVALID_ARGUMENT
+    assert call(Hkv=65536) == BC_ERR_UNSUPPORTED
     assert call(T=0, q=None, k=None, qo=None, ko=None) == BC_OK
     assert call(H=0, Hkv=0, q=None, k=None, qo=None, ko=None) == BC_OK
 
@@ -57,6 +59,10 @@ def test_append_argument_errors(lib, no_gpu):  # noqa: F811
     assert call(slots=None) == BC_ERR_INVALID_ARGUMENT
     assert call(qo=None) == BC_ERR_INVALID_ARGUMENT
     assert call(H=0, q=None, qo=None, qw=X) == BC_ERR_INVALID_ARGUMENT
+    assert call(H=65536) == BC_ERR_UNSUPPORTED
+    assert call(qo=P(0x1008)) == BC_ERR_INVALID_ARGUMENT
+    assert call(kb=P(0x1004)) == BC_ERR_INVALID_ARGUMENT
+    assert call(vr=P(0x1002)) == BC_ERR_INVALID_ARGUMENT
     assert call(T=0, q=None, k=None, v=None, slots=None) == BC_OK
 
 
@@ -105,6 +111,8 @@ def test_paged_attention_argument_errors(lib, no_gpu):  # noqa: F811
     assert call(lens=None) == BC_ERR_INVALID_ARGUMENT
     assert call(tables=None) == BC_ERR_INVALID_ARGUMENT
     assert call(kb=None) == BC_ERR_INVALID_ARGUMENT
+    assert call(kr=P(0x1008)) == BC_ERR_INVALID_ARGUMENT
+    assert call(ws=P(0x10008)) == BC_ERR_INVALID_ARGUMENT
     assert call(B=0, q=None, out=None) == BC_OK
 
 
