@@ -64,17 +64,17 @@ struct AttnArgs {
 // chooses chunk from the lengths, so that the launch is planned without knowing
 // them and a captured call follows them.  unit_slots units (times the head
 // groups) run at once.  Eight candidates aim at half to two rounds of them, and
-// the one with the least rounds * (mean unit + kUnitFixed) is taken (the fixed
-// work of a unit, its query preparation, merge and first loads, is that of four
-// tiles), as far as its units fit the launched ones (unit_most); chunk is at
-// least unit_tiles and at most kUnitTiles (a wave holds its tiles' places in one
-// register), which always fits.  unit_tiles = 0: unit b is sequence b.  Each wave
-// finds its unit by itself, and one notes the sequences' units for the merge.  (64
-// sequences of 128 to 32768 keys, 32/8 heads, by an earlier form of the kernel: 119
-// us; the candidates taken alone 112 to 124, those that do not fit 180; one equal
-// range of tiles per slot, across sequences, 159: two segments in most ranges, each
-// with the fixed work and none beside another's loop.)
-constexpr int kUnitTiles = 256, kUnitFixed = 4, kUnitRounds = 2;
+// the cheapest is taken (the fixed work of a unit, its query preparation, merge and
+// first loads, counts as kUnitFixed tiles), as far as its units fit the launched
+// ones (unit_most); chunk is at least unit_tiles and at most kUnitTiles (a wave
+// holds its tiles' places in one register), which always fits.  unit_tiles = 0:
+// unit b is sequence b.  Each wave finds its unit by itself, and one notes the
+// sequences' units for the merge.  (64 sequences of 128 to 32768 keys, 32/8 heads,
+// 478 MB: 93 us; by rounds times the mean unit 111, since few units of unequal
+// length leave a tail; 64 of 6144 keys, 528 MB, 90 and 104.  One equal range of
+// tiles per slot, across sequences, took 40 us more than units: two segments in
+// most ranges, each with the fixed work and none beside another's loop.)
+constexpr int kUnitTiles = 256, kUnitFixed = 6, kUnitRounds = 2;
 struct PagedUnit {
     int b, len;        // (b < 0: no such unit)
     int first, tiles;  // the unit's tiles, counted from key0
@@ -130,8 +130,10 @@ __device__ __forceinline__ int paged_chunk(const AttnArgs& a, int lane, int& own
     units += __builtin_amdgcn_ds_swizzle(units, 0x201F);
     units += __builtin_amdgcn_ds_swizzle(units, 0x401F);
     units += __builtin_amdgcn_ds_bpermute(4 * (lane ^ 32), units);
-    const float rounds = ceilf((float)units / (float)a.unit_slots);
-    const float tiles = rounds * ((float)total / (float)max(units, 1) + (float)kUnitFixed);
+    // (one round: its longest unit; more: the slots' share, and half a unit at the end)
+    const float tiles = units <= a.unit_slots
+                            ? (float)(chunk + kUnitFixed)
+                            : ((float)total + (float)kUnitFixed * (float)units) / (float)a.unit_slots + 0.5f * (float)chunk;
     uint32_t cost[1] = {~((uint32_t)fminf(16.0f * tiles, 268435455.0f) << 3 | (uint32_t)cand)};
     if (units > a.unit_most) cost[0] = 0;
     wave_umax(cost);

@@ -475,7 +475,9 @@ __host__ __device__ constexpr bool k_on_mfma(int G, int mode) {
 // PG: a paged cache (kv_rows pages times kv heads, kv_stride the page size): the
 // workgroup takes work unit blockIdx.y (PagedUnit) of kv head and group
 // blockIdx.x; a tile lies in one page, so each tile's loads go through buffer
-// resources of its own, over its keys alone.
+// resources of its own, over its keys alone.  8 x 32 heads of 65536 keys (2.8 GB):
+// 433 us, 6.5 TB/s, 418 in a ring; signs alone (604 MB) 101 and 87: the resources
+// weigh on tiles of 2.3 KB.
 //
 // The scalar arguments (14 dwords) come in registers with the wave (kernarg
 // preloading: a launch's first read of its argument memory takes about a

@@ -23,7 +23,8 @@ using bc::MODE_COMP;
 // The merge of a sequence's units, and of the shared prefix's `splits` partials per
 // row: PARTS waves per (sequence, query head), each over every PARTS-th partial
 // (lane = partial for the factors, lanes = dims for the sums), joined in LDS.
-// Bound: the latency of its three loads in turn (units, maxima, sums).
+// Bound: the latency of its three loads in turn (units, maxima, sums): 5 us for 256
+// to 2048 rows of 5 to 10 partials, 7 with the prefix's.
 template <int D, int PARTS>
 __global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t* out, const float* prefix, int splits) {
     constexpr int N = (D + 63) / 64;     // dims of a lane
@@ -126,10 +127,10 @@ size_t note_bytes(int batch) { return ((size_t)batch * sizeof(int2) + 15) & ~(si
 // Whether the shared prefix has its own kernel: where the sequences would read 192 MB
 // or more of it.  Less, and its launch and its partials cost more than the bytes
 // (whole calls, 200 keys more per sequence, us without and with it; residual
-// planes, 32/8 heads of 128: 32768 keys, 4 sequences 38 and 42, 8 52 and 45, 32 140
-// and 77; 8192 keys, 16 sequences 36 and 43, 32 50 and 52; 32/32 heads, 2048 keys, 8
-// sequences 24 and 25, 32 57 and 40; signs only, 32/8 heads, 32768 keys, 16
-// sequences 40 and 48, 32 61 and 58).  BITCACHE_SHARED=1 and =0 choose it always and never (tuning).
+// planes, 32/8 heads of 128: 32768 keys, 4 sequences 34 and 42, 8 50 and 43, 32 144
+// and 75; 8192 keys, 16 sequences 33 and 43, 32 48 and 49; 32/32 heads, 2048 keys, 8
+// sequences 20 and 25, 32 43 and 37; signs only, 32/8 heads, 32768 keys, 16
+// sequences 37 and 48, 32 58 and 56).  BITCACHE_SHARED=1 and =0 choose it always and never (tuning).
 bool prefix_pays(int mode, int64_t batch, int n_kv_heads, int64_t shared_len, int d) {
     if (const char* e = getenv("BITCACHE_SHARED")) return e[0] == '1';
     const int64_t pair = 2 * (mode == MODE_BINARY ? d / 8 + 2 : d / 8 + 2 + d / 2 + 2);
@@ -166,9 +167,12 @@ PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len
     const int cu = bc::device_cu_count();
     int fit = bc::paged_wgs_per_cu(mode, d, p.G);
     if (fit <= 0) fit = 3;
-    // (four workgroups a CU keep the memory busy; five or more cut long sequences finer:
-    // signs of 64 sequences of 8192 keys, 32/8 heads, 54 us for 43.5)
-    if (fit > 4) fit = 4;
+    // (two workgroups a CU keep the memory busy with residual planes, four with signs
+    // alone, and a round of more cuts sequences finer: residual planes, 64 sequences of
+    // 500 to 16000 keys, 32/8 heads of 64, 50 us, 55 with 3 or 4; 64 of 6144 keys of 128,
+    // 90 and 96; signs, 64 of 8192 keys, 32/8 heads of 128, 41 us, with 3 49, with 2 52)
+    const int most_fit = mode == MODE_BINARY ? 4 : 2;
+    if (fit > most_fit) fit = most_fit;
     p.unit_slots = (int)(((int64_t)fit * cu + p.groups - 1) / p.groups);
     // (at least two tiles a wave, one where that leaves CUs idle)
     p.unit_tiles = (int64_t)batch * p.groups * ((tiles + 7) / 8) < cu ? 4 : 8;
