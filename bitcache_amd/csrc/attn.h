@@ -55,6 +55,7 @@ struct AttnArgs {
     int width, n_pages, page_tiles, key0, max_len;
     int unit_tiles;   // see PagedUnit; 0: one unit per sequence
     int unit_slots, unit_most;
+    int unit_each;    // units of every sequence, kUnitTiles each; 0: cut by the lengths
     int2* units;      // each sequence's first unit and how many it has
     int bf16;         // queries and outputs are bf16
 };
@@ -68,7 +69,8 @@ struct AttnArgs {
 // first loads, counts as kUnitFixed tiles), as far as its units fit the launched
 // ones (unit_most); chunk is at least unit_tiles and at most kUnitTiles (a wave
 // holds its tiles' places in one register), which always fits.  unit_tiles = 0:
-// unit b is sequence b.  Each wave finds its unit by itself, and one notes the
+// unit b is sequence b; unit_each: unit b unit_each + i is the i-th of sequence b (a
+// large batch, whose lengths would take each wave too long to go through).  Each wave finds its unit by itself, and one notes the
 // sequences' units for the merge.  (64 sequences of 128 to 32768 keys, 32/8 heads,
 // 478 MB: 93 us; by rounds times the mean unit 111, since few units of unequal
 // length leave a tail; 64 of 6144 keys, 528 MB, 90 and 104.  One equal range of
@@ -145,6 +147,12 @@ __device__ __forceinline__ PagedUnit paged_unit(const AttnArgs& a, int unit, int
     if (a.unit_tiles == 0) {
         const int len = __builtin_amdgcn_readfirstlane(a.lens[unit]);
         return PagedUnit{unit, len, 0, paged_tiles(a, len)};
+    }
+    if (a.unit_each > 0) {
+        const int b = unit / a.unit_each, first = (unit - b * a.unit_each) * kUnitTiles;
+        const int len = __builtin_amdgcn_readfirstlane(a.lens[b]), tiles = paged_tiles(a, len);
+        if (first >= tiles) return PagedUnit{-1, 0, 0, 0};
+        return PagedUnit{b, len, first, min(tiles - first, kUnitTiles)};
     }
     int own;
     const int chunk = paged_chunk(a, lane, own);

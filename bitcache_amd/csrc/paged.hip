@@ -36,8 +36,10 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t
     const bool live = row < (int64_t)a.B * a.Hq;
     const int b = live ? (int)(row / a.Hq) : 0, h = live ? (int)(row - (int64_t)b * a.Hq) : 0;
     // (without units: all keys are the prefix's)
-    const int2 u = a.unit_most > 0 ? a.units[b] : make_int2(0, 0);
     const int len = a.lens[b];
+    int2 u = make_int2(0, 0);
+    if (a.unit_each > 0) u = make_int2(b * a.unit_each, (bc::paged_tiles(a, len) + bc::kUnitTiles - 1) / bc::kUnitTiles);
+    else if (a.unit_most > 0) u = a.units[b];
     const int64_t own_step = (int64_t)a.Hq * (D + 2), prefix_step = own_step * a.B;
     const float* const own = a.ws + (int64_t)u.x * own_step + (int64_t)h * (D + 2);
     const float* const shared = prefix + ((int64_t)b * a.Hq + h) * (D + 2);
@@ -114,7 +116,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(AttnArgs a, uint16_t
 
 struct PagedPlan {
     int G, groups;     // query heads of a workgroup, workgroups per sequence and unit
-    int unit_tiles, unit_slots;
+    int unit_tiles, unit_slots, unit_each;
     int units;         // at most
     // the shared prefix's kernel (splits 0: the prefix is attended as own keys)
     int splits, tiles_per, nc, row_groups;
@@ -179,6 +181,18 @@ PagedPlan plan(int mode, int batch, int n_heads, int n_kv_heads, int max_seq_len
     const int64_t most = (int64_t)batch * ((tiles + p.unit_tiles - 1) / p.unit_tiles);
     int64_t units = bc::paged_unit_most(p.unit_slots, batch, batch * tiles);
     if (units > most) units = most;
+    // A large batch is even enough by itself, and its lengths take each wave long to go
+    // through: equal units of every sequence instead (us by the lengths and in equal units,
+    // 500 to 4000 keys, 32/8 heads of 128: 128 sequences 77 and 77, 400 215 and 186, 1024 585
+    // and 418; 100 to 8000 keys, 8/2 heads: 128 sequences 33 and 67, 700 121 and 116, 1024
+    // 173 and 145; signs, 64 to 20000 keys, 32/8 heads: 256 98 and 147, 700 296 and 328, 1024
+    // 499 and 444).
+    // (as far as a launch holds them)
+    const int64_t each = (tiles + bc::kUnitTiles - 1) / bc::kUnitTiles;
+    if ((batch > 4 * p.unit_slots || batch > 640) && units > 0 && batch * each <= 65535) {
+        p.unit_each = (int)each;
+        units = batch * each;
+    }
     p.units = (int)units;
     p.own_bytes = note_bytes(batch) + (size_t)units * n_heads * (d + 2) * sizeof(float);
     p.bytes = p.own_bytes + (size_t)p.splits * batch * n_heads * (d + 2) * sizeof(float);
@@ -271,6 +285,7 @@ extern "C" int bc_paged_attention(const void* q, const void* k_bin, const void* 
     a.unit_tiles = p.unit_tiles;
     a.unit_slots = p.unit_slots;
     a.unit_most = p.units;
+    a.unit_each = p.unit_each;
     // (the workspace: the sequences' units, their partials, the prefix's)
     a.units = (int2*)workspace;
     a.bf16 = dtype == BC_BF16;

@@ -411,3 +411,23 @@ def test_two_streams_at_once(F):
                 got.append(c())
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(alone, got))
+
+
+@pytest.mark.parametrize("B,H,Hkv,d,residual", [(700, 2, 1, 64, True), (641, 2, 2, 32, False), (300, 8, 8, 64, True)])
+def test_large_batches(F, B, H, Hkv, d, residual):
+    """Batches whose units are equal ones of every sequence, several of long sequences; a bad
+    page, and a length over the bound, give NaN there alone; with a shared prefix too."""
+    lens = [(37 * i) % 400 for i in range(B)]
+    lens[3], lens[B - 1], lens[64] = 16385, 20000, 33000
+    q, blobs, tables, lens_t = setup(B, lens, H, Hkv, d, 64, residual, torch.float16)
+    want = check(F, q, blobs, tables, lens_t, 64, Hkv, 40000)
+    tables[3, 200], lens_t[65] = -7, 40001
+    got = F.paged_attention(q, *blobs, tables, lens_t, 40000, 64, n_kv_heads=Hkv)
+    assert bool(torch.isnan(got[3]).all()) and bool(torch.isnan(got[65]).all())
+    rest = torch.ones(B, dtype=torch.bool, device="cuda")
+    rest[3] = rest[65] = False
+    assert torch.equal(got[rest], want[rest])
+    lens = [64 + n for n in lens[:400]]
+    if d == 64:
+        q, blobs, tables, lens_t = setup(B + 1, lens, H, Hkv, d, 64, residual, torch.float16, shared=64)
+        check(F, q, blobs, tables, lens_t, 64, Hkv, 40000, shared=64)
