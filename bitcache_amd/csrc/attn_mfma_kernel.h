@@ -653,7 +653,7 @@ void attn_mfma_kernel(const uint16_t* q, const uint8_t* k_signs, const uint8_t* 
             // (into a scalar register: a resource made of a vector register takes a loop over the
             // lanes per load: 64 sequences of 128 to 32768 keys 119 us, 116 without)
             const int keys = __builtin_amdgcn_readfirstlane(min(max(key_end - t0, 0), 64));
-            const int i = (t0 - key_begin) / (64 * NW) & 63;   // (past the range: any tile, no keys)
+            const int i = (int)((uint32_t)(t0 - key_begin) / (64 * NW)) & 63;   // (past the range: any tile, no keys)
             const int64_t v = (int64_t)(uint32_t)__builtin_amdgcn_readlane(tile_at, i) * 64;
             return __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)plane + v * rb), (short)0, keys * rb, kBufWord3);
         } else {
