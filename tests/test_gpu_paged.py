@@ -394,7 +394,7 @@ def test_queries_at_odd_elements(F, shared):
         F.paged_attention(q, moved, *blobs[1:], tables, lens_t, max(lens), 64, n_kv_heads=2, shared_len=shared)
 
 
-def test_two_streams_at_once(F):
+def test_two_streams_merging_units(F):
     """Calls on two streams, each with its own workspace, and the same calls alone."""
     calls = []
     for seed in (60, 61):
